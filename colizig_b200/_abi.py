@@ -15,7 +15,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 # COLIZIG_LIBRARY overrides the in-tree library (to compare builds); unset in normal use.
 LIB_PATH = os.environ.get("COLIZIG_LIBRARY") or os.path.join(HERE, "libcolizig_cuda.so")
 
-# the six symbols of the reference surface (gpu.zig:84-89) + the MoE-level ones
+# the six symbols of the reference surface (gpu.zig:84-89) + the MoE-level and attention ones
 REFERENCE_SYMBOLS = (
     "colizig_cuda_init",
     "colizig_cuda_device_name",
@@ -48,6 +48,11 @@ MOE_SYMBOLS = (
     "colizig_cuda_ep_set_combine",
     "colizig_cuda_kernel_timer",
     "colizig_cuda_kernel_timer_read",
+    "colizig_cuda_attn_append",
+    "colizig_cuda_attn_decode_workspace",
+    "colizig_cuda_attn_decode",
+    "colizig_cuda_attn_prefill",
+    "colizig_cuda_attn_check",
 )
 
 # callback types of colizig_cuda_debug_watch_wait (query / async error, abort)
@@ -60,6 +65,9 @@ COLIZIG_EP_SHARDED = 4
 COLIZIG_SHARED_BF16 = 8
 COLIZIG_X_F32 = 0
 COLIZIG_X_BF16 = 1
+COLIZIG_KV_BF16 = 0
+COLIZIG_KV_E4M3 = 1
+COLIZIG_ATTN_MAX_BATCH = 4096
 
 ERRORS = {
     -1: "bad arguments / not initialised",
@@ -72,6 +80,7 @@ ERRORS = {
     -8: "shape not supported",
     -9: "NCCL / expert-parallel error",
     -10: "checkpoint file missing, unreadable or malformed, or a tensor missing",
+    -11: "an index in device memory pointed outside its buffer",
 }
 
 
@@ -100,6 +109,24 @@ class MoeExpert(ctypes.Structure):
         ("up_s", ctypes.c_void_p),
         ("down_w", ctypes.c_void_p),
         ("down_s", ctypes.c_void_p),
+    ]
+
+
+class KvCacheC(ctypes.Structure):
+    """colizig_kv_cache."""
+
+    _fields_ = [
+        ("k", ctypes.c_void_p),
+        ("v", ctypes.c_void_p),
+        ("k_scale", ctypes.c_void_p),
+        ("v_scale", ctypes.c_void_p),
+        ("k_page_stride", ctypes.c_uint64),
+        ("v_page_stride", ctypes.c_uint64),
+        ("pages", ctypes.c_uint32),
+        ("page_size", ctypes.c_uint32),
+        ("kv_heads", ctypes.c_uint32),
+        ("head_dim", ctypes.c_uint32),
+        ("dtype", ctypes.c_uint32),
     ]
 
 
@@ -182,6 +209,19 @@ def load(path: str = LIB_PATH) -> ctypes.CDLL:
         L.colizig_cuda_debug_error_bits.argtypes = [ctypes.c_void_p]
         L.colizig_cuda_debug_watch_wait.restype = i32
         L.colizig_cuda_debug_watch_wait.argtypes = [WATCH_QUERY, WATCH_QUERY, WATCH_ABORT, ctypes.c_void_p, i32]
+        kv, f32 = ctypes.POINTER(KvCacheC), ctypes.c_float
+        L.colizig_cuda_attn_append.restype = i32
+        L.colizig_cuda_attn_append.argtypes = [kv, vp, vp, vp, i32, i32, u32, u64, u64, u64, vp, vp, vp, u32, u32, vp,
+                                               vp, f32, vp, vp, vp, vp]
+        L.colizig_cuda_attn_decode_workspace.restype = ctypes.c_size_t
+        L.colizig_cuda_attn_decode_workspace.argtypes = []
+        L.colizig_cuda_attn_decode.restype = i32
+        L.colizig_cuda_attn_decode.argtypes = [kv, vp, u64, i32, u32, vp, u32, u64, vp, f32, vp, vp, vp]
+        L.colizig_cuda_attn_prefill.restype = i32
+        L.colizig_cuda_attn_prefill.argtypes = [vp, vp, vp, u64, u64, u64, i32, i32, i32, u32, u32, u32, vp, vp, f32,
+                                                vp, vp]
+        L.colizig_cuda_attn_check.restype = i32
+        L.colizig_cuda_attn_check.argtypes = [vp]
         _lib = L
         return L
 

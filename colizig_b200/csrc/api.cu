@@ -184,6 +184,7 @@ struct Ctx {
     HostBuf mm_xh, mm_yh;  // pinned staging of colizig_cuda_matmul_fp8's x and y (up to kHostStageCap bytes)
     HostBuf io_xh;    // pinned staging of the tokens (host-pointer forward, up to kHostStageCap bytes)
     uint32_t* sync = nullptr;
+    uint32_t* attn_err = nullptr;  // the attention calls' error word
     // expert parallelism (one process per GPU)
     bool ep_on = false;
     int ep_rank = 0, ep_world = 1;
@@ -484,6 +485,7 @@ void shutdown_locked() {
                       &g.sh_tmp, &g.sh_send, &g.sh_recv, &g.sh_x, &g.sh_ridx, &g.sh_rgates, &g.sh_part, &g.sh_back})
         b->release();
     if (g.sync) cudaFree(g.sync);
+    if (g.attn_err) cudaFree(g.attn_err);
     for (cudaEvent_t e : g.tm_ev) cudaEventDestroy(e);
     if (g.stream) cudaStreamDestroy(g.stream);
     g = Ctx{};
@@ -503,6 +505,15 @@ int init_locked(int device) {
     g.num_sms = prop.multiProcessorCount;
     g.dev = device;
     if (cudaStreamCreateWithFlags(&g.stream, cudaStreamNonBlocking) != cudaSuccess) return -4;
+    // allocated here, not on first use: an attention call may be inside a stream capture
+    if (cudaMalloc(&g.attn_err, sizeof(uint32_t)) != cudaSuccess ||
+        cudaMemset(g.attn_err, 0, sizeof(uint32_t)) != cudaSuccess || cudaStreamSynchronize(nullptr) != cudaSuccess) {
+        if (g.attn_err) cudaFree(g.attn_err);
+        g.attn_err = nullptr;
+        cudaStreamDestroy(g.stream);
+        g.stream = nullptr;
+        return -4;
+    }
     g.budget = 0;  // keyed store disabled until set (colizig_cuda.cu:184)
     g.inited = true;
     return CZ_OK;
@@ -1777,4 +1788,179 @@ CZ_EXPORT int colizig_cuda_moe_forward_noalloc(uint32_t layer, const void* x, in
         if (cudaMemsetAsync(sync + 1, 0, sizeof(uint32_t), st) != cudaSuccess) return CZ_ELAUNCH;
     }
     return CZ_OK;
+}
+
+// ============================ Part 3: attention ============================
+
+namespace {
+
+// Checks a caller's cache and makes the kernels' view of it.
+int kv_view(const colizig_kv_cache* c, cz::KvView& v) {
+    if (!c || !c->k || !c->v || !aligned16(c->k) || !aligned16(c->v)) return CZ_EARGS;
+    if (c->dtype != COLIZIG_KV_BF16 && c->dtype != COLIZIG_KV_E4M3) return CZ_EARGS;
+    const uint64_t elt = c->dtype == COLIZIG_KV_BF16 ? 2 : 1;
+    if (elt == 2 && (c->k_scale || c->v_scale)) return CZ_EARGS;
+    if (c->pages < 1 || c->kv_heads < 1 || c->page_size < 16 || c->page_size % 16 || c->page_size > 65536 ||
+        c->pages > 0x7fffffffu || c->kv_heads > 65535 || (c->head_dim != 64 && c->head_dim != 128))
+        return CZ_ESHAPE;
+    const uint64_t page = (uint64_t)c->kv_heads * c->page_size * c->head_dim;
+    if (c->k_page_stride < page || c->v_page_stride < page || c->k_page_stride * elt % 16 ||
+        c->v_page_stride * elt % 16)
+        return CZ_EARGS;
+    v.k = reinterpret_cast<uint8_t*>(c->k);
+    v.v = reinterpret_cast<uint8_t*>(c->v);
+    v.k_scale = c->k_scale;
+    v.v_scale = c->v_scale;
+    v.k_page = c->k_page_stride;
+    v.v_page = c->v_page_stride;
+    v.pages = c->pages;
+    v.page_size = c->page_size;
+    v.kv_heads = c->kv_heads;
+    v.head_dim = c->head_dim;
+    v.e4m3 = elt == 1;
+    return CZ_OK;
+}
+
+// A row of `heads` heads at `stride` elements: rows do not overlap and start on 16 bytes.
+bool row_ok(uint64_t stride, uint64_t heads, uint64_t dim, uint64_t elt) {
+    return stride >= heads * dim && stride * elt % 16 == 0;
+}
+
+}  // namespace
+
+CZ_EXPORT int colizig_cuda_attn_append(const colizig_kv_cache* cache, const void* q, const void* k, const void* v,
+                                       int x_dtype, int T, uint32_t q_heads, uint64_t q_stride, uint64_t k_stride,
+                                       uint64_t v_stride, const int32_t* positions, const int64_t* slots,
+                                       const float* rope, uint32_t rope_len, uint32_t rot_dim, const float* q_norm,
+                                       const float* k_norm, float eps, void* q_out, void* k_out, void* v_out,
+                                       void* stream) {
+    CsrGuard _csr;
+    std::lock_guard<std::mutex> lk(g_mu);
+    if (!g.inited || T < 0 || (x_dtype != COLIZIG_X_F32 && x_dtype != COLIZIG_X_BF16)) return CZ_EARGS;
+    cz::AppendParams p{};
+    if (const int rc = kv_view(cache, p.kv)) return rc;
+    if (T == 0) return CZ_OK;
+    const uint32_t D = p.kv.head_dim, hk = p.kv.kv_heads;
+    if (q_heads < 1 || q_heads > 65535 || q_heads % hk || rot_dim % 16 || rot_dim > D) return CZ_ESHAPE;
+    if (!q || !k || !v || !slots || !q_out || !aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(q_out) ||
+        !aligned16(k_out) || !aligned16(v_out) || !aligned16(q_norm) || !aligned16(k_norm) || !aligned16(rope))
+        return CZ_EARGS;
+    if ((rope == nullptr) != (rot_dim == 0) || (rope && (!positions || rope_len < 1))) return CZ_EARGS;
+    const uint64_t elt = x_dtype == COLIZIG_X_BF16 ? 2 : 4;
+    if (!row_ok(q_stride, q_heads, D, elt) || !row_ok(k_stride, hk, D, elt) || !row_ok(v_stride, hk, D, elt))
+        return CZ_EARGS;
+    p.q = q;
+    p.k = k;
+    p.v = v;
+    p.x_bf16 = elt == 2;
+    p.T = T;
+    p.q_heads = q_heads;
+    p.q_stride = q_stride;
+    p.k_stride = k_stride;
+    p.v_stride = v_stride;
+    p.positions = positions;
+    p.slots = slots;
+    p.rope = rope;
+    p.rope_len = rope_len;
+    p.rot = rot_dim;
+    p.q_norm = q_norm;
+    p.k_norm = k_norm;
+    p.eps = eps;
+    p.q_out = reinterpret_cast<uint16_t*>(q_out);
+    p.k_out = reinterpret_cast<uint16_t*>(k_out);
+    p.v_out = reinterpret_cast<uint16_t*>(v_out);
+    p.err = g.attn_err;
+    cudaSetDevice(g.dev);
+    return cz::attn_append_launch(p, reinterpret_cast<cudaStream_t>(stream));
+}
+
+CZ_EXPORT size_t colizig_cuda_attn_decode_workspace(void) {
+    std::lock_guard<std::mutex> lk(g_mu);
+    return g.inited ? cz::attn_decode_workspace_bytes(g.num_sms) : 0;
+}
+
+CZ_EXPORT int colizig_cuda_attn_decode(const colizig_kv_cache* cache, const void* q, uint64_t q_stride, int B,
+                                       uint32_t q_heads, const int32_t* table, uint32_t table_width,
+                                       uint64_t table_stride, const int32_t* lens, float scale, void* out,
+                                       void* workspace, void* stream) {
+    CsrGuard _csr;
+    std::lock_guard<std::mutex> lk(g_mu);
+    if (!g.inited || B < 0) return CZ_EARGS;
+    cz::AttnDecodeParams p{};
+    if (const int rc = kv_view(cache, p.kv)) return rc;
+    if (B == 0) return CZ_OK;
+    if (B > COLIZIG_ATTN_MAX_BATCH || q_heads < 1 || q_heads > 65535 || q_heads % p.kv.kv_heads) return CZ_ESHAPE;
+    if (!q || !table || !lens || !out || !workspace || !aligned16(q) || !aligned16(out) ||
+        (reinterpret_cast<uintptr_t>(workspace) & 255u) || table_width < 1 || table_stride < table_width ||
+        !row_ok(q_stride, q_heads, p.kv.head_dim, 2))
+        return CZ_EARGS;
+    // a sequence's length has to fit 32 bits
+    if ((uint64_t)table_width * p.kv.page_size > 0x7fffff00u) return CZ_ESHAPE;
+    p.q = reinterpret_cast<const uint16_t*>(q);
+    p.q_stride = q_stride;
+    p.B = B;
+    p.q_heads = q_heads;
+    p.table = table;
+    p.table_width = table_width;
+    p.table_stride = table_stride;
+    p.lens = lens;
+    p.scale = scale;
+    p.out = reinterpret_cast<uint16_t*>(out);
+    p.workspace = workspace;
+    p.err = g.attn_err;
+    cudaSetDevice(g.dev);
+    return cz::attn_decode_launch(p, g.num_sms, reinterpret_cast<cudaStream_t>(stream));
+}
+
+CZ_EXPORT int colizig_cuda_attn_prefill(const void* q, const void* k, const void* v, uint64_t q_stride,
+                                        uint64_t k_stride, uint64_t v_stride, int Tq, int Tk, int B, uint32_t q_heads,
+                                        uint32_t kv_heads, uint32_t head_dim, const int32_t* cu_q, const int32_t* cu_k,
+                                        float scale, void* out, void* stream) {
+    CsrGuard _csr;
+    std::lock_guard<std::mutex> lk(g_mu);
+    if (!g.inited || Tq < 0 || Tk < 0 || B < 0) return CZ_EARGS;
+    if (Tq == 0 || B == 0) return CZ_OK;
+    if (B > COLIZIG_ATTN_MAX_BATCH || (head_dim != 64 && head_dim != 128) || kv_heads < 1 || kv_heads > 65535 ||
+        q_heads < 1 || q_heads > 65535 || q_heads % kv_heads)
+        return CZ_ESHAPE;
+    if (!q || !cu_q || !cu_k || !out || !aligned16(q) || !aligned16(out) || !row_ok(q_stride, q_heads, head_dim, 2))
+        return CZ_EARGS;
+    if (Tk > 0 && (!k || !v || !aligned16(k) || !aligned16(v) || !row_ok(k_stride, kv_heads, head_dim, 2) ||
+                   !row_ok(v_stride, kv_heads, head_dim, 2)))
+        return CZ_EARGS;
+    cz::AttnPrefillParams p{};
+    p.q = reinterpret_cast<const uint16_t*>(q);
+    p.k = reinterpret_cast<const uint16_t*>(k);
+    p.v = reinterpret_cast<const uint16_t*>(v);
+    p.q_stride = q_stride;
+    p.k_stride = k_stride;
+    p.v_stride = v_stride;
+    p.Tq = Tq;
+    p.Tk = Tk;
+    p.B = B;
+    p.q_heads = q_heads;
+    p.kv_heads = kv_heads;
+    p.head_dim = head_dim;
+    p.cu_q = cu_q;
+    p.cu_k = cu_k;
+    p.scale = scale;
+    p.out = reinterpret_cast<uint16_t*>(out);
+    p.err = g.attn_err;
+    cudaSetDevice(g.dev);
+    return cz::attn_prefill_launch(p, g.num_sms, reinterpret_cast<cudaStream_t>(stream));
+}
+
+CZ_EXPORT int colizig_cuda_attn_check(void* stream) {
+    CsrGuard _csr;
+    std::lock_guard<std::mutex> lk(g_mu);
+    if (!g.inited) return CZ_EARGS;
+    cudaSetDevice(g.dev);
+    cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+    uint32_t err = 0;
+    if (cudaMemcpyAsync(&err, g.attn_err, sizeof err, cudaMemcpyDeviceToHost, st) != cudaSuccess) return CZ_ED2H;
+    if (const int rc = stream_sync(st)) return rc;
+    if (!err) return CZ_OK;
+    if (cudaMemsetAsync(g.attn_err, 0, sizeof err, st) != cudaSuccess) return CZ_ELAUNCH;
+    if (const int rc = stream_sync(st)) return rc;
+    return CZ_EINDEX;
 }

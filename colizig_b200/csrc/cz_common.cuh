@@ -20,6 +20,7 @@ enum {
     CZ_ETIMEOUT = -7,
     CZ_ESHAPE = -8,
     CZ_ENCCL = -9,
+    CZ_EINDEX = -11,
 };
 
 // Device error-word bits (OR-ed together by any CTA that gives up a wait).

@@ -189,6 +189,66 @@ int shb_launch(const ShbParams& p, bool gate_up, cudaStream_t st);
 int fp8_matmul_launch(float* y, const float* x, const uint8_t* w, const float* scales, int S, int I, int O,
                       cudaStream_t stream);
 
+// ---- attention over a paged key/value cache (attn_append.cu, attn_decode.cu, attn_prefill.cu) ----
+
+constexpr uint32_t kAttnErrIndex = 1u;  // attention error word: an index in device memory was out of range
+
+// The caller's cache as the kernels see it (include/colizig_cuda.h, colizig_kv_cache).
+struct KvView {
+    uint8_t *k, *v;
+    const float *k_scale, *v_scale;  // E4M3: per kv head, or null
+    uint64_t k_page, v_page;         // page strides in elements
+    uint32_t pages, page_size, kv_heads, head_dim;
+    int e4m3;
+};
+
+struct AppendParams {
+    KvView kv;
+    const void *q, *k, *v;
+    int x_bf16, T;
+    uint32_t q_heads;
+    uint64_t q_stride, k_stride, v_stride;
+    const int32_t* positions;
+    const int64_t* slots;
+    const float* rope;  // [rope_len][rot]: rot/2 cosines, rot/2 sines (null: no rotation)
+    uint32_t rope_len, rot;
+    const float *q_norm, *k_norm;
+    float eps;
+    uint16_t *q_out, *k_out, *v_out;  // bf16 bits; k_out, v_out nullable
+    uint32_t* err;
+};
+int attn_append_launch(const AppendParams& p, cudaStream_t stream);
+
+struct AttnDecodeParams {
+    KvView kv;
+    const uint16_t* q;  // bf16 [B][q_heads][head_dim]
+    uint64_t q_stride;
+    int B;
+    uint32_t q_heads;
+    const int32_t* table;
+    uint32_t table_width;
+    uint64_t table_stride;
+    const int32_t* lens;
+    float scale;
+    uint16_t* out;
+    void* workspace;
+    uint32_t* err;
+};
+size_t attn_decode_workspace_bytes(int num_sms);
+int attn_decode_launch(const AttnDecodeParams& p, int num_sms, cudaStream_t stream);
+
+struct AttnPrefillParams {
+    const uint16_t *q, *k, *v;  // bf16 rows
+    uint64_t q_stride, k_stride, v_stride;
+    int Tq, Tk, B;
+    uint32_t q_heads, kv_heads, head_dim;
+    const int32_t *cu_q, *cu_k;
+    float scale;
+    uint16_t* out;
+    uint32_t* err;
+};
+int attn_prefill_launch(const AttnPrefillParams& p, int num_sms, cudaStream_t stream);
+
 int debug_expf_launch(const float* x, float* y, size_t n, cudaStream_t stream);
 
 }  // namespace cz

@@ -13,6 +13,9 @@
  * softmax/top-k, token-to-expert gather, gate/up with SiLU*mul, down, weighted
  * combine — on resident weights in one call.
  *
+ * Part 3 adds the attention between the FP8 projections: rotation and cache write,
+ * attention of one new token over the paged cache, attention over whole prompts.
+ *
  * Return codes (reference convention, colizig_cuda.cu:228-284, extended):
  *    0 ok
  *   -1 bad arguments / not initialised       -2 device allocation failed
@@ -22,6 +25,7 @@
  *      still usable and the next call starts clean)
  *   -8 shape not supported by this build     -9 NCCL / expert-parallel error
  *  -10 checkpoint file missing, unreadable or malformed, or a tensor missing
+ *  -11 an index in device memory pointed outside its buffer (Part 3)
  *
  * Threading: one process-wide context, internally serialised by a mutex.
  * Ownership: callers own every buffer they pass; no pointer is retained after
@@ -302,6 +306,93 @@ int colizig_cuda_debug_error_bits(uint32_t* bits);
  * (aborted: deadline or error); -1 for a null callback. */
 int colizig_cuda_debug_watch_wait(int (*query)(void*), int (*async_error)(void*), void (*abort_comm)(void*),
                                   void* ctx, int timeout_ms);
+
+/* ---- Part 3: attention over a paged key/value cache ---------------------
+ *
+ * What the decoder layer runs between its FP8 projections (q/k/v before, o after;
+ * src/qwen3moe/attn.zig:46-78): the position rotation and the cache write, attention
+ * of one new token per sequence, attention over whole prompts.  Every pointer is a
+ * device pointer on the device of colizig_cuda_init; every call is queued on `stream`
+ * (NULL = the default stream), allocates nothing, keeps nothing and can be captured
+ * into a CUDA graph.  Rows are 16-byte aligned: base pointers and row strides (given
+ * in elements) are multiples of 16 bytes, head h of a row starts head_dim * h further
+ * on.  head_dim is 64 or 128; q_heads is a multiple of kv_heads.
+ *
+ * Indices that live in device memory (positions, slots, page tables, lengths, sequence
+ * bounds) are checked by the kernels: one that points outside its buffer is never
+ * followed, and the call sets a word that colizig_cuda_attn_check reports as -11. */
+
+#define COLIZIG_KV_BF16 0u
+#define COLIZIG_KV_E4M3 1u
+
+/* A paged cache of the caller's: page p, head h, row r is head_dim elements at
+ * k + (p * k_page_stride) + (h * page_size + r) * head_dim.  page_size is a multiple of
+ * 16, page strides are at least kv_heads * page_size * head_dim elements (more when
+ * keys and values alternate in one allocation).  E4M3: element = code * scale[h]
+ * (NULL = 1); BF16 caches take no scales. */
+typedef struct colizig_kv_cache {
+    void* k;
+    void* v;
+    const float* k_scale;
+    const float* v_scale;
+    uint64_t k_page_stride;
+    uint64_t v_page_stride;
+    uint32_t pages;
+    uint32_t page_size;
+    uint32_t kv_heads;
+    uint32_t head_dim;
+    uint32_t dtype;
+} colizig_kv_cache;
+
+/* Norm, rotation and cache write of T tokens' projections, x_dtype COLIZIG_X_F32 or
+ * COLIZIG_X_BF16, rows of q_heads (kv_heads) heads at the given strides:
+ *   y = x / sqrt(mean(x^2) + eps) * norm          per head (q_norm / k_norm f32 [head_dim], NULL = y = x)
+ *   (y[i], y[i+R/2]) turned by the angle of (positions[t], i), i < R/2, R = rot_dim
+ * for q and k; v is taken as it is.  rope is f32 [rope_len][rot_dim]: R/2 cosines, then
+ * R/2 sines of a position's angles; rot_dim a multiple of 16 and at most head_dim (0 and
+ * rope NULL: no rotation, positions unused).  q goes to q_out bf16 [T, q_heads,
+ * head_dim]; k and v go to row slots[t] % page_size of page slots[t] / page_size
+ * (negative: not cached; two tokens of one call never share a slot), rounded once to
+ * the cache's type (E4M3: x / scale saturated at 448).  k_out / v_out (nullable): packed
+ * bf16 [T, kv_heads, head_dim] copies for colizig_cuda_attn_prefill.  No output may
+ * overlap an input.  0, -1 (arguments, alignment), -8 (shape), -4 (launch). */
+int colizig_cuda_attn_append(const colizig_kv_cache* cache, const void* q, const void* k, const void* v,
+                             int x_dtype, int T, uint32_t q_heads, uint64_t q_stride, uint64_t k_stride,
+                             uint64_t v_stride, const int32_t* positions, const int64_t* slots, const float* rope,
+                             uint32_t rope_len, uint32_t rot_dim, const float* q_norm, const float* k_norm,
+                             float eps, void* q_out, void* k_out, void* v_out, void* stream);
+
+/* Attention of one new token per sequence over the cache:
+ *   out[b,h] = sum_j softmax_j(scale * q[b,h] . k_j) v_j,   j < lens[b]
+ * with key j of sequence b in page table[b][j / page_size].  q bf16 [B, q_heads,
+ * head_dim] at q_stride elements a sequence, table int32 [B, table_width] at
+ * table_stride, lens int32 [B]; out bf16 [B, q_heads, head_dim].  A sequence of length 0
+ * gives zeros.  Rows of a page past the length may hold anything, NaN included.
+ * B is at most COLIZIG_ATTN_MAX_BATCH.  workspace: colizig_cuda_attn_decode_workspace
+ * bytes, 256-byte aligned and zeroed once before its first use; each call leaves it
+ * ready for the next.  Calls that may overlap in time need a workspace each. */
+#define COLIZIG_ATTN_MAX_BATCH 4096
+size_t colizig_cuda_attn_decode_workspace(void);
+int colizig_cuda_attn_decode(const colizig_kv_cache* cache, const void* q, uint64_t q_stride, int B,
+                             uint32_t q_heads, const int32_t* table, uint32_t table_width, uint64_t table_stride,
+                             const int32_t* lens, float scale, void* out, void* workspace, void* stream);
+
+/* Causal attention over packed prompts: sequence b holds query rows cu_q[b] ..
+ * cu_q[b+1] of q and key rows cu_k[b] .. cu_k[b+1] of k and v, all bf16.  Queries are the
+ * sequence's last tokens: query i sees the keys j <= i + nk - nq (nq, nk the
+ * sequence's row counts), and gives zeros when there is none.  q [Tq, q_heads,
+ * head_dim], k and v [Tk, kv_heads, head_dim] at the given row strides; cu_q, cu_k
+ * int32 [B + 1], cu[0] = 0, ascending; out bf16 [Tq, q_heads, head_dim].  A key row
+ * must be finite where any query of its own sequence is computed; other sequences'
+ * rows never reach a result.  0, -1, -8 (shape), -4. */
+int colizig_cuda_attn_prefill(const void* q, const void* k, const void* v, uint64_t q_stride, uint64_t k_stride,
+                              uint64_t v_stride, int Tq, int Tk, int B, uint32_t q_heads, uint32_t kv_heads,
+                              uint32_t head_dim, const int32_t* cu_q, const int32_t* cu_k, float scale, void* out,
+                              void* stream);
+
+/* Reads and clears the attention calls' error word (synchronises `stream`): 0, or -11
+ * when a call since the last read met an index outside its buffer. */
+int colizig_cuda_attn_check(void* stream);
 
 #ifdef __cplusplus
 }
