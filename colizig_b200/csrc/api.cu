@@ -1894,8 +1894,8 @@ CZ_EXPORT int colizig_cuda_attn_decode(const colizig_kv_cache* cache, const void
         (reinterpret_cast<uintptr_t>(workspace) & 255u) || table_width < 1 || table_stride < table_width ||
         !row_ok(q_stride, q_heads, p.kv.head_dim, 2))
         return CZ_EARGS;
-    // a sequence's length has to fit 32 bits
-    if ((uint64_t)table_width * p.kv.page_size > 0x7fffff00u) return CZ_ESHAPE;
+    // a sequence's length, and the steps past its end, have to fit 31 bits
+    if ((uint64_t)table_width * p.kv.page_size > 0x7fff0000u) return CZ_ESHAPE;
     p.q = reinterpret_cast<const uint16_t*>(q);
     p.q_stride = q_stride;
     p.B = B;
@@ -1962,5 +1962,5 @@ CZ_EXPORT int colizig_cuda_attn_check(void* stream) {
     if (!err) return CZ_OK;
     if (cudaMemsetAsync(g.attn_err, 0, sizeof err, st) != cudaSuccess) return CZ_ELAUNCH;
     if (const int rc = stream_sync(st)) return rc;
-    return CZ_EINDEX;
+    return err & cz::kAttnErrWait ? CZ_ETIMEOUT : CZ_EINDEX;
 }

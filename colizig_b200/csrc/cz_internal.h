@@ -191,7 +191,25 @@ int fp8_matmul_launch(float* y, const float* x, const uint8_t* w, const float* s
 
 // ---- attention over a paged key/value cache (attn_append.cu, attn_decode.cu, attn_prefill.cu) ----
 
-constexpr uint32_t kAttnErrIndex = 1u;  // attention error word: an index in device memory was out of range
+// Attention error word.
+constexpr uint32_t kAttnErrIndex = 1u;  // an index in device memory was out of range (-11)
+constexpr uint32_t kAttnErrWait = 2u;   // a bounded wait gave up (-7)
+
+// cuTensorMapEncodeTiled, looked up once (null when the driver has none).
+typedef CUresult (*EncodeTiled)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+inline EncodeTiled encode_tiled() {
+    static EncodeTiled fn = nullptr;
+    if (!fn) {
+        void* f = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) == cudaSuccess &&
+            q == cudaDriverEntryPointSuccess)
+            fn = reinterpret_cast<EncodeTiled>(f);
+    }
+    return fn;
+}
 
 // The caller's cache as the kernels see it (include/colizig_cuda.h, colizig_kv_cache).
 struct KvView {

@@ -390,8 +390,9 @@ int colizig_cuda_attn_prefill(const void* q, const void* k, const void* v, uint6
                               uint32_t head_dim, const int32_t* cu_q, const int32_t* cu_k, float scale, void* out,
                               void* stream);
 
-/* Reads and clears the attention calls' error word (synchronises `stream`): 0, or -11
- * when a call since the last read met an index outside its buffer. */
+/* Reads and clears the attention calls' error word (synchronises `stream`): 0, -11 when a
+ * call since the last read met an index outside its buffer, -7 when a bounded wait in
+ * a kernel gave up. */
 int colizig_cuda_attn_check(void* stream);
 
 #ifdef __cplusplus
