@@ -1890,6 +1890,7 @@ CZ_EXPORT int colizig_cuda_attn_decode(const colizig_kv_cache* cache, const void
     if (const int rc = kv_view(cache, p.kv)) return rc;
     if (B == 0) return CZ_OK;
     if (B > COLIZIG_ATTN_MAX_BATCH || q_heads < 1 || q_heads > 65535 || q_heads % p.kv.kv_heads) return CZ_ESHAPE;
+    if (!(scale > 0.f) || scale > 3.4e38f) return CZ_EARGS;
     if (!q || !table || !lens || !out || !workspace || !aligned16(q) || !aligned16(out) ||
         (reinterpret_cast<uintptr_t>(workspace) & 255u) || table_width < 1 || table_stride < table_width ||
         !row_ok(q_stride, q_heads, p.kv.head_dim, 2))
@@ -1923,6 +1924,7 @@ CZ_EXPORT int colizig_cuda_attn_prefill(const void* q, const void* k, const void
     if (B > COLIZIG_ATTN_MAX_BATCH || (head_dim != 64 && head_dim != 128) || kv_heads < 1 || kv_heads > 65535 ||
         q_heads < 1 || q_heads > 65535 || q_heads % kv_heads)
         return CZ_ESHAPE;
+    if (!(scale > 0.f) || scale > 3.4e38f) return CZ_EARGS;
     if (!q || !cu_q || !cu_k || !out || !aligned16(q) || !aligned16(out) || !row_ok(q_stride, q_heads, head_dim, 2))
         return CZ_EARGS;
     if (Tk > 0 && (!k || !v || !aligned16(k) || !aligned16(v) || !row_ok(k_stride, kv_heads, head_dim, 2) ||

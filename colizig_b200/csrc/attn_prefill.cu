@@ -1,7 +1,21 @@
 // Causal attention over packed prompts: query i of sequence b (nq queries, nk keys,
 // aligned at their ends) sees the keys j <= i + nk - nq;
-//   out = sum_j p_j v_j,  p = softmax_j(scale q . k_j),  zeros when it sees none.
-// One warp per (query, head), running maximum and sum of the softmax in f32.
+//   out = sum_j p_j v_j,  p = softmax_j(scale q . k_j),  zeros when it sees none,
+// over tiles of 128 keys with a running maximum m and sum l (f32):
+//   S = Q K^T,  P = 2^(c S - c m),  l += rowsum P,  O += P V,  c = scale log2(e).
+//
+// Bound by the tensor pipe (4 D flops per visible pair) with the exponentials (one per
+// pair and head, 16 a clock and SM) close behind.  Both products run on tcgen05 with
+// their accumulators in TMEM: S and O of two 128-row query tiles fill its 512 columns, so
+// that one tile's softmax runs under the other's products; P replaces S in place as
+// bf16 and is the second product's A operand straight from TMEM.
+//
+// A query tile packs the G query heads of a key/value head: row = token * G + head, 128 / G
+// tokens.  Keys and values are read once for all of them, a short prompt still fills
+// the tile (16 tokens of 8 heads), and the diagonal wastes at most 16 of 128 keys there.
+//
+// Warps: 0-3 and 4-7 softmax of query tile 0 and 1 (a thread a row), 8 TMA loads, 9 MMA
+// issue.  Blocks take tiles from the largest key count down, so the last to finish are short.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -12,64 +26,575 @@
 namespace cz {
 namespace {
 
-constexpr int kWarps = 4;
+constexpr int kThreads = 320;
+constexpr int kKeys = 128;     // keys per tile
+constexpr uint32_t kTmemCols = 512;
+// A row's old maximum stays in use until a new one is more than this many powers of two
+// above it: P and l then grow to at most 2^8, far inside f32 and bf16, and most tiles
+// rescale nothing.  The result does not depend on it (o and l share the factor).
+constexpr float kSlack = 8.f;
+
+struct PrefillArgs {
+    CUtensorMap qmap, kmap, vmap;  // [rows][heads][D] in boxes of 64 columns
+    AttnPrefillParams p;
+    int group, pack, tokens;       // query heads per kv head; heads and tokens of a query tile
+    int htiles;                    // passes over a group's heads
+};
 
 template <int D>
-__global__ void __launch_bounds__(kWarps * 32) attn_prefill_kernel(const AttnPrefillParams p) {
-    constexpr int N = D / 32;
+struct Cfg {
+    static constexpr int NX = D / 64;                  // 128-byte column blocks
+    static constexpr int QBYTES = 128 * D * 2;
+    static constexpr int KVBYTES = kKeys * D * 2;
+    static constexpr int STAGES = (227 * 1024 - 2048 - 2 * QBYTES) / KVBYTES > 8 ? 8 : (227 * 1024 - 2048 - 2 * QBYTES) / KVBYTES;
+    static constexpr int SMEM = 1024 + 2 * QBYTES + STAGES * KVBYTES;
+    static constexpr uint32_t OCOL = 256;              // O of tile i at OCOL + i * 128, S of tile i at i * 128
+};
+
+struct Bars {
+    uint64_t qfull[2], full[8], empty[8], sfull[2], pready[2], odone[2], drain;
+    uint32_t tmem;
+    int abort, never;
+    int q0, nq, k0, nk, tile;  // this block's sequence and query tile pair (tile < 0: none)
+};
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+__device__ __forceinline__ void tma3d(uint32_t dst, const CUtensorMap* m, int x, int head, int row, uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], "
+        "[%5];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(m)), "r"(x), "r"(head), "r"(row), "r"(smem_u32(bar))
+        : "memory");
+}
+// Shared-memory operand descriptors, 128-byte swizzle: K-major rows of 128 bytes (8-row
+// groups 1024 bytes apart), or MN-major (V: keys are rows of 64 dims; 8-key groups 1024 bytes
+// apart, the next 64 dims `chunk` bytes on).
+__device__ __forceinline__ uint64_t desc_k(uint32_t a) {
+    return (uint64_t)((a >> 4) & 0x3FFF) | ((uint64_t)1 << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) |
+           ((uint64_t)2 << 61);
+}
+__device__ __forceinline__ uint64_t desc_mn(uint32_t a, uint32_t chunk) {
+    return (uint64_t)((a >> 4) & 0x3FFF) | ((uint64_t)(chunk >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
+           ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+// kind::f16, bf16 x bf16 -> f32; bmn: B is MN-major.
+__host__ __device__ constexpr uint32_t idesc(int M, int N, bool bmn) {
+    return (1u << 4) | (1u << 7) | (1u << 10) | (bmn ? 1u << 16 : 0u) | ((uint32_t)(N >> 3) << 17) |
+           ((uint32_t)(M >> 4) << 24);
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t acc) {
+    asm volatile(
+        "{\n.reg .pred p;\nsetp.ne.u32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d),
+        "l"(a), "l"(b), "r"(id), "r"(acc)
+        : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t id, uint32_t acc) {
+    asm volatile(
+        "{\n.reg .pred p;\nsetp.ne.u32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(d),
+        "r"(a), "l"(b), "r"(id), "r"(acc)
+        : "memory");
+}
+__device__ __forceinline__ void commit(uint64_t* bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
+                 : "memory");
+}
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+__device__ __forceinline__ void ld32(uint32_t* r, uint32_t a) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,"
+        "%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+          "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+          "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(a)
+        : "memory");
+}
+__device__ __forceinline__ void st32(uint32_t a, const uint32_t* r) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,"
+        "%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};" ::"r"(r[0]),
+        "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+        "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]),
+        "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]),
+        "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(a)
+        : "memory");
+}
+__device__ __forceinline__ void st16(uint32_t a, const uint32_t* r) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::"r"(
+            r[0]),
+        "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+        "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(a)
+        : "memory");
+}
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+
+// A sequence's bounds; false (and reported) when they leave the buffers.
+__device__ __forceinline__ bool bounds(const AttnPrefillParams& p, int b, int& q0, int& nq, int& k0, int& nk) {
+    q0 = __ldg(p.cu_q + b);
+    k0 = __ldg(p.cu_k + b);
+    const int q1 = __ldg(p.cu_q + b + 1), k1 = __ldg(p.cu_k + b + 1);
+    nq = q1 - q0;
+    nk = k1 - k0;
+    if (q0 < 0 || q1 < q0 || q1 > p.Tq || k0 < 0 || k1 < k0 || k1 > p.Tk) {
+        nq = nk = 0;
+        return false;
+    }
+    return true;
+}
+// How many of a sequence's query tile pairs (of `step` tokens) reach key x or a later one; all of
+// them for x <= 0.  The pair's reach is its last token's, as if the last pair were full.
+__device__ __forceinline__ int reach(int nq, int nk, int step, int x) {
+    const int n = (nq + step - 1) / step;
+    const int y = x - (nk - nq);  // first pair i with (i + 1) step >= y
+    if (x <= 0 || y <= step) return n;
+    return max(0, n - ((y + step - 1) / step - 1));
+}
+
+// One warp: the query tile pair of rank `rank`, longest reach first.
+__device__ void pick(const AttnPrefillParams& p, int step, int rank, Bars& B) {
     const int lane = threadIdx.x & 31;
-    const uint64_t item = (uint64_t)blockIdx.x * kWarps + (threadIdx.x >> 5);
-    if (item >= (uint64_t)p.Tq * p.q_heads) return;
-    const int t = (int)(item / p.q_heads);
-    const uint32_t h = (uint32_t)(item % p.q_heads), kh = h / (p.q_heads / p.kv_heads);
-    int b = 0;
-    while (b < p.B && __ldg(p.cu_q + b + 1) <= t) ++b;
-    int n = 0, k0 = 0;
-    if (b < p.B) {
-        const int q0 = __ldg(p.cu_q + b), q1 = __ldg(p.cu_q + b + 1);
-        k0 = __ldg(p.cu_k + b);
-        const int k1 = __ldg(p.cu_k + b + 1);
-        if (q0 < 0 || q1 > p.Tq || k0 < 0 || k1 < k0 || k1 > p.Tk) {
-            if (lane == 0) atomicOr(p.err, kAttnErrIndex);
-        } else {
-            n = t - q0 + 1 + (k1 - k0) - (q1 - q0);
+    auto count = [&](int x) {
+        int c = 0;
+        for (int b = lane; b < p.B; b += 32) {
+            int q0, nq, k0, nk;
+            bounds(p, b, q0, nq, k0, nk);
+            c += reach(nq, nk, step, x);
+        }
+        return (int)__reduce_add_sync(0xffffffffu, (unsigned)c);
+    };
+    int tile = -1, q0 = 0, nq = 0, k0 = 0, nk = 0;
+    if (p.B == 1) {
+        const bool ok = bounds(p, 0, q0, nq, k0, nk);
+        if (!ok && rank == 0 && lane == 0) atomicOr(p.err, kAttnErrIndex);
+        const int n = (nq + step - 1) / step;
+        tile = rank < n ? n - 1 - rank : -1;
+    } else {
+        int top = 0;  // past every reach
+        for (int b = lane; b < p.B; b += 32) {
+            const bool ok = bounds(p, b, q0, nq, k0, nk);
+            if (!ok && rank == 0) atomicOr(p.err, kAttnErrIndex);
+            top = max(top, nk + step);
+        }
+        top = (int)__reduce_max_sync(0xffffffffu, (unsigned)top) + 1;
+        if (count(0) > rank) {
+            int lo = 0, hi = top;  // count(lo) > rank >= count(hi)
+            while (hi - lo > 1) {
+                const int mid = lo + (hi - lo) / 2;
+                if (count(mid) > rank) lo = mid;
+                else hi = mid;
+            }
+            int left = rank - count(hi);  // which of the pairs that reach lo but not hi
+            for (int b0 = 0; b0 < p.B; b0 += 32) {
+                const int b = b0 + lane;
+                int c = 0;
+                q0 = nq = k0 = nk = 0;
+                if (b < p.B) {
+                    bounds(p, b, q0, nq, k0, nk);
+                    c = reach(nq, nk, step, lo) - reach(nq, nk, step, hi);
+                }
+                int inc = c;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const int v = __shfl_up_sync(0xffffffffu, inc, o);
+                    if (lane >= o) inc += v;
+                }
+                const unsigned hit = __ballot_sync(0xffffffffu, left < inc);
+                if (hit) {
+                    const int src = __ffs(hit) - 1;
+                    const int n = (nq + step - 1) / step;
+                    const int t = n - reach(nq, nk, step, lo) + (left - (inc - c));
+                    tile = __shfl_sync(0xffffffffu, t, src);
+                    q0 = __shfl_sync(0xffffffffu, q0, src);
+                    nq = __shfl_sync(0xffffffffu, nq, src);
+                    k0 = __shfl_sync(0xffffffffu, k0, src);
+                    nk = __shfl_sync(0xffffffffu, nk, src);
+                    break;
+                }
+                left -= __shfl_sync(0xffffffffu, inc, 31);
+            }
         }
     }
-    float q[N], o[N], m = -INFINITY, l = 0.f;
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-        q[i] = bf16_bits_to_f32(__ldg(p.q + t * p.q_stride + (uint64_t)h * D + lane * N + i));
-        o[i] = 0.f;
+    if (lane == 0) {
+        B.tile = tile;
+        B.q0 = q0;
+        B.nq = nq;
+        B.k0 = k0;
+        B.nk = nk;
     }
-    for (int j = 0; j < n; ++j) {
-        const uint16_t* kr = p.k + (uint64_t)(k0 + j) * p.k_stride + (uint64_t)kh * D + lane * N;
-        const uint16_t* vr = p.v + (uint64_t)(k0 + j) * p.v_stride + (uint64_t)kh * D + lane * N;
-        float d = 0.f;
-#pragma unroll
-        for (int i = 0; i < N; ++i) d = __fmaf_rn(q[i], bf16_bits_to_f32(__ldg(kr + i)), d);
-        const float s = warp_sum(d) * p.scale;
-        const float mn = fmaxf(m, s), a = m == mn ? 1.f : expf(m - mn), w = s == mn ? 1.f : expf(s - mn);
-#pragma unroll
-        for (int i = 0; i < N; ++i) o[i] = __fmaf_rn(w, bf16_bits_to_f32(__ldg(vr + i)), o[i] * a);
-        l = __fmaf_rn(l, a, w);
-        m = mn;
+}
+
+template <int D>
+__global__ void __launch_bounds__(kThreads, 1) attn_prefill_kernel(const __grid_constant__ PrefillArgs A) {
+    using C = Cfg<D>;
+    const AttnPrefillParams& p = A.p;
+    extern __shared__ uint8_t raw[];
+    uint8_t* sq = raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u);
+    uint8_t* skv = sq + 2 * C::QBYTES;
+    __shared__ Bars B;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int heads = (int)p.kv_heads * A.htiles;
+    const int hi = (int)(blockIdx.x % heads), rank = (int)(blockIdx.x / heads);
+    const int kh = hi / A.htiles, head0 = (hi % A.htiles) * A.pack;  // first query head of the group's pass
+
+    if (warp == 0) pick(p, 2 * A.tokens, rank, B);
+    if (warp == 8 && lane == 0) {
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&B.qfull[i], 1);
+            mbar_init(&B.sfull[i], 1);
+            mbar_init(&B.pready[i], 4);
+            mbar_init(&B.odone[i], 1);
+        }
+        for (int i = 0; i < C::STAGES; ++i) {
+            mbar_init(&B.full[i], 1);
+            mbar_init(&B.empty[i], 1);
+        }
+        mbar_init(&B.drain, 1);
+        B.abort = B.never = 0;
+        fence_mbarrier_init();
+        prefetch_tensormap(&A.qmap);
+        prefetch_tensormap(&A.kmap);
+        prefetch_tensormap(&A.vmap);
     }
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-        const __nv_bfloat16 v = __float2bfloat16_rn(l > 0.f ? o[i] / l : 0.f);
-        p.out[((uint64_t)t * p.q_heads + h) * D + lane * N + i] = *reinterpret_cast<const uint16_t*>(&v);
+    if (warp == 9) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&B.tmem)),
+                     "r"(kTmemCols)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
+    fence_before();
+    __syncthreads();
+    fence_after();
+    const uint32_t tmem = B.tmem;
+    volatile int* abort = &B.abort;
+    const int tile = B.tile, nq = B.nq, nk = B.nk, q0 = B.q0, k0 = B.k0;
+
+    // key tiles of each query tile: up to its last token's limit
+    int n[2], tok[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        tok[i] = tile * 2 * A.tokens + i * A.tokens;
+        const int last = min(nq, tok[i] + A.tokens) - 1 + nk - nq;
+        n[i] = tile < 0 || tok[i] >= nq || last < 0 ? 0 : last / kKeys + 1;
+    }
+    const int nmax = max(n[0], n[1]);
+
+    auto gave_up = [&]() {
+        *abort = 1;
+        atomicOr(p.err, kAttnErrWait);
+    };
+
+    if (tile < 0) {
+        // more blocks than query tiles (the grid is sized without reading the bounds)
+    } else if (warp == 8) {
+        // ---------------- loads ----------------
+        if (lane == 0 && nmax > 0) {
+            const uint32_t qbytes = (uint32_t)(A.tokens * A.pack) * 128 * C::NX;
+            auto load_q = [&](int i) {
+                if (n[i] == 0) return;
+                mbar_arrive_expect_tx(&B.qfull[i], qbytes);
+#pragma unroll
+                for (int x = 0; x < C::NX; ++x)
+                    tma3d(smem_u32(sq + i * C::QBYTES + x * 128 * 128), &A.qmap, x * 64, kh * A.group + head0,
+                          q0 + tok[i], &B.qfull[i]);
+            };
+            int issued = 0;
+            auto load_kv = [&](const CUtensorMap* m, int j) {
+                const int s = issued % C::STAGES;
+                if (issued >= C::STAGES &&
+                    !mbar_wait_bounded(&B.empty[s], ((issued / C::STAGES) & 1) ^ 1, abort)) {
+                    gave_up();
+                    return false;
+                }
+                mbar_arrive_expect_tx(&B.full[s], C::KVBYTES);
+#pragma unroll
+                for (int x = 0; x < C::NX; ++x)
+                    tma3d(smem_u32(skv + s * C::KVBYTES + x * kKeys * 128), m, x * 64, kh, k0 + j * kKeys, &B.full[s]);
+                ++issued;
+                return true;
+            };
+            load_q(0);
+            bool ok = load_kv(&A.kmap, 0);
+            load_q(1);
+            ok = ok && load_kv(&A.vmap, 0);
+            for (int j = 1; j < nmax && ok; ++j) ok = load_kv(&A.kmap, j) && load_kv(&A.vmap, j);
+            // no copy stays in flight behind the block's end (all have landed unless a wait gave up)
+            for (int i = max(0, issued - C::STAGES); i < issued; ++i)
+                if (!mbar_wait_bounded(&B.full[i % C::STAGES], (i / C::STAGES) & 1, &B.never)) gave_up();
+        }
+        __syncwarp();
+    } else if (warp == 9) {
+        // ---------------- MMA ----------------
+        constexpr uint32_t IDS = idesc(128, kKeys, false), IDO = idesc(128, D, true);
+        auto wait = [&](uint64_t* bar, uint32_t parity) {
+            bool ok = true;
+            if (lane == 0) {
+                ok = mbar_wait_bounded(bar, parity, abort);
+                if (!ok) gave_up();
+            }
+            return (bool)__shfl_sync(0xffffffffu, ok, 0);
+        };
+        auto stage = [&](int use) { return skv + (use % C::STAGES) * C::KVBYTES; };
+        auto wait_kv = [&](int use) { return wait(&B.full[use % C::STAGES], (use / C::STAGES) & 1); };
+        auto qk = [&](int i, int j) {  // S_i = Q_i K_j^T
+            if (lane == 0) {
+                const uint32_t qa = smem_u32(sq + i * C::QBYTES), ka = smem_u32(stage(2 * j));
+#pragma unroll
+                for (int k = 0; k < D / 16; ++k)
+                    mma_ss(tmem + i * 128, desc_k(qa + (k / 4) * 128 * 128) + (k % 4) * 2,
+                           desc_k(ka + (k / 4) * kKeys * 128) + (k % 4) * 2, IDS, k > 0);
+                commit(&B.sfull[i]);
+            }
+            __syncwarp();
+        };
+        auto done_kv = [&](int use) {
+            if (lane == 0) commit(&B.empty[use % C::STAGES]);
+            __syncwarp();
+        };
+        bool ok = nmax == 0 || wait_kv(0);
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+            if (ok && n[i] > 0) {
+                ok = wait(&B.qfull[i], 0);
+                if (ok) qk(i, 0);
+            }
+        if (ok && nmax > 0) done_kv(0);
+        for (int j = 0; j < nmax && ok; ++j) {
+            // keys of this tile that belong to the sequence; products past them are left out, and the
+            // rows that fill up the last 16 (a neighbour's, of any value) are cleared
+            const int valid = min(kKeys, nk - j * kKeys), ksteps = (valid + 15) / 16;
+            ok = wait_kv(2 * j + 1);
+            if (!ok) break;
+            if (valid & 15) {
+                uint8_t* v = stage(2 * j + 1);
+                for (int i = lane; i < (ksteps * 16 - valid) * 8 * C::NX; i += 32) {
+                    const int r = valid + i / (8 * C::NX), c = i % (8 * C::NX);
+                    *reinterpret_cast<uint4*>(v + (c >> 3) * kKeys * 128 + r * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
+                }
+                fence_proxy_async_smem();
+                __syncwarp();
+            }
+            const bool more = j + 1 < nmax;
+            if (more) {
+                ok = wait_kv(2 * j + 2);
+                if (!ok) break;
+            }
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                if (j >= n[i]) continue;
+                ok = wait(&B.pready[i], j & 1);
+                if (!ok) break;
+                fence_after();
+                if (lane == 0) {
+                    const uint32_t va = smem_u32(stage(2 * j + 1));
+                    for (int k = 0; k < ksteps; ++k)
+                        mma_ts(tmem + C::OCOL + i * 128, tmem + i * 128 + k * 8, desc_mn(va + k * 2048, kKeys * 128),
+                               IDO, j > 0 || k > 0);
+                    if (j + 1 == n[i]) commit(&B.odone[i]);
+                }
+                __syncwarp();
+                if (j + 1 < n[i]) qk(i, j + 1);  // into S_i: in order behind the product that reads P_i from it
+            }
+            if (!ok) break;
+            done_kv(2 * j + 1);
+            if (more) done_kv(2 * j + 2);
+        }
+        if (lane == 0) {  // every product has finished before TMEM is given back
+            commit(&B.drain);
+            if (!mbar_wait_bounded(&B.drain, 0, &B.never)) gave_up();
+        }
+        __syncwarp();
+    } else {
+        // ---------------- softmax: a thread a row ----------------
+        const int i = warp >> 2;
+        const int r = (warp & 3) * 32 + lane;
+        const int lt = r / A.pack, lh = r % A.pack;
+        const int t = (i ? tok[1] : tok[0]) + lt;
+        const bool live = lt < A.tokens && t < nq && head0 + lh < A.group;
+        const int tiles = i ? n[1] : n[0];
+        const int lim0 = (i ? tok[1] : tok[0]) + nk - nq;  // the tile's first token's limit
+        const int lim = live ? t + nk - nq : 0x7fffffff;
+        const uint32_t quad = (uint32_t)((warp & 3) * 32) << 16;
+        const uint32_t sa = tmem + quad + i * 128, oa = tmem + quad + C::OCOL + i * 128;
+        const float c = p.scale * 1.4426950408889634f;
+        float m = -INFINITY, l = 0.f;
+        bool ok = true;
+        for (int j = 0; j < tiles; ++j) {
+            ok = mbar_wait_bounded(&B.sfull[i], j & 1, abort);
+            if (!__all_sync(0xffffffffu, ok)) {
+                gave_up();
+                ok = false;
+                break;
+            }
+            fence_after();
+            // S is read twice, 32 columns at a time (maximum, then weights): held whole, it would
+            // take 128 registers
+            const bool diagonal = j * kKeys + kKeys - 1 > lim0;
+            const int cut = lim - j * kKeys;  // columns past it are not seen
+            auto hide = [&](uint32_t* s, int x0) {
+#pragma unroll
+                for (int x = 0; x < 32; ++x)
+                    if (x0 + x > cut) s[x] = 0xff800000u;
+            };
+            float mx[4] = {m, m, m, m};
+            {
+                uint32_t s[2][32];
+                ld32(s[0], sa);
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                    wait_ld();
+                    if (x < 3) ld32(s[(x + 1) & 1], sa + (x + 1) * 32);
+                    if (diagonal) hide(s[x & 1], x * 32);
+#pragma unroll
+                    for (int y = 0; y < 32; ++y) mx[y & 3] = fmaxf(mx[y & 3], __uint_as_float(s[x & 1][y]));
+                }
+            }
+            const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+            if (j == 0) {
+                m = top;
+            } else if (__any_sync(0xffffffffu, (top - m) * c > kSlack)) {
+                // the products into O behind this tile's S have finished: S's completion covers them
+                const float a = top == m ? 1.f : ex2((m - top) * c);
+                m = top;
+                l *= a;
+#pragma unroll
+                for (int x = 0; x < D / 32; ++x) {
+                    uint32_t o[32];
+                    ld32(o, oa + x * 32);
+                    wait_ld();
+#pragma unroll
+                    for (int y = 0; y < 32; ++y) o[y] = __float_as_uint(__uint_as_float(o[y]) * a);
+                    st32(oa + x * 32, o);
+                }
+            }
+            const float mc = m == -INFINITY ? 0.f : m * c;
+            float sum[2] = {0.f, 0.f};
+            {
+                uint32_t s[2][32];
+                ld32(s[0], sa);
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                    wait_ld();
+                    if (x < 3) ld32(s[(x + 1) & 1], sa + (x + 1) * 32);
+                    if (diagonal) hide(s[x & 1], x * 32);
+                    uint32_t pk[16];
+#pragma unroll
+                    for (int y = 0; y < 16; ++y) {
+                        const float e0 = ex2(__fmaf_rn(__uint_as_float(s[x & 1][2 * y]), c, -mc));
+                        const float e1 = ex2(__fmaf_rn(__uint_as_float(s[x & 1][2 * y + 1]), c, -mc));
+                        sum[0] += e0;
+                        sum[1] += e1;
+                        pk[y] = pack_bf16(e0, e1);  // the second product's operand; its sums stay in f32
+                    }
+                    st16(sa + x * 16, pk);  // over columns that have been read
+                }
+            }
+            l += sum[0] + sum[1];
+            wait_st();
+            fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&B.pready[i]);
+        }
+        if (ok && tiles > 0) {
+            ok = mbar_wait_bounded(&B.odone[i], 0, abort);
+            if (!__all_sync(0xffffffffu, ok)) {
+                gave_up();
+                ok = false;
+            }
+            fence_after();
+        }
+        if (ok) {
+            const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
+            uint4* dst = reinterpret_cast<uint4*>(
+                p.out + ((uint64_t)(q0 + t) * p.q_heads + (uint64_t)kh * A.group + head0 + lh) * D);
+#pragma unroll
+            for (int x = 0; x < D / 32; ++x) {
+                uint32_t o[32];
+                if (tiles > 0) {
+                    ld32(o, oa + x * 32);
+                    wait_ld();
+                }
+                if (live) {
+#pragma unroll
+                    for (int y = 0; y < 4; ++y) {
+                        uint32_t w[4];
+#pragma unroll
+                        for (int z = 0; z < 4; ++z)
+                            w[z] = inv == 0.f ? 0u
+                                              : pack_bf16(__uint_as_float(o[y * 8 + 2 * z]) * inv,
+                                                          __uint_as_float(o[y * 8 + 2 * z + 1]) * inv);
+                        dst[x * 4 + y] = make_uint4(w[0], w[1], w[2], w[3]);
+                    }
+                }
+                __syncwarp();
+            }
+        }
+        fence_before();
+    }
+    __syncthreads();
+    if (warp == 9)
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
+}
+
+bool make_map(CUtensorMap* map, const uint16_t* base, uint64_t rows, uint64_t heads, uint64_t dim, uint64_t stride,
+              uint32_t box_heads, uint32_t box_rows) {
+    const EncodeTiled fn = encode_tiled();
+    if (!fn) return false;
+    const cuuint64_t dims[3] = {dim, heads, rows};
+    const cuuint64_t strides[2] = {dim * 2, stride * 2};
+    const cuuint32_t box[3] = {64, box_heads, box_rows};
+    const cuuint32_t one[3] = {1, 1, 1};
+    return fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<uint16_t*>(base), dims, strides, box, one,
+              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int D>
+int launch(const PrefillArgs& a, uint32_t grid, cudaStream_t st) {
+    static bool set = false;  // the library's lock is held
+    if (!set) {
+        if (cudaFuncSetAttribute(attn_prefill_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 Cfg<D>::SMEM) != cudaSuccess)
+            return CZ_ELAUNCH;
+        set = true;
+    }
+    attn_prefill_kernel<D><<<grid, kThreads, Cfg<D>::SMEM, st>>>(a);
+    return cudaGetLastError() == cudaSuccess ? CZ_OK : CZ_ELAUNCH;
 }
 
 }  // namespace
 
 int attn_prefill_launch(const AttnPrefillParams& p, int, cudaStream_t st) {
-    const uint32_t grid = (uint32_t)(((uint64_t)p.Tq * p.q_heads + kWarps - 1) / kWarps);
-    if (p.head_dim == 128)
-        attn_prefill_kernel<128><<<grid, kWarps * 32, 0, st>>>(p);
-    else
-        attn_prefill_kernel<64><<<grid, kWarps * 32, 0, st>>>(p);
-    return cudaGetLastError() == cudaSuccess ? CZ_OK : CZ_ELAUNCH;
+    if (p.Tk == 0)  // no query sees a key
+        return cudaMemsetAsync(p.out, 0, (size_t)p.Tq * p.q_heads * p.head_dim * 2, st) == cudaSuccess ? CZ_OK
+                                                                                                      : CZ_ELAUNCH;
+    PrefillArgs a{};
+    a.p = p;
+    a.group = (int)(p.q_heads / p.kv_heads);
+    a.htiles = (a.group + 127) / 128;
+    a.pack = (a.group + a.htiles - 1) / a.htiles;
+    a.tokens = 128 / a.pack;
+    const uint64_t grid = ((uint64_t)p.Tq / (2 * a.tokens) + p.B) * p.kv_heads * a.htiles;
+    if (grid > 0x7fffffffu) return CZ_ESHAPE;
+    if (!make_map(&a.qmap, p.q, p.Tq, p.q_heads, p.head_dim, p.q_stride, a.pack, a.tokens) ||
+        !make_map(&a.kmap, p.k, p.Tk, p.kv_heads, p.head_dim, p.k_stride, 1, kKeys) ||
+        !make_map(&a.vmap, p.v, p.Tk, p.kv_heads, p.head_dim, p.v_stride, 1, kKeys))
+        return CZ_ESHAPE;
+    return p.head_dim == 128 ? launch<128>(a, (uint32_t)grid, st) : launch<64>(a, (uint32_t)grid, st);
 }
 
 }  // namespace cz

@@ -316,7 +316,7 @@ int colizig_cuda_debug_watch_wait(int (*query)(void*), int (*async_error)(void*)
  * (NULL = the default stream), allocates nothing, keeps nothing and can be captured
  * into a CUDA graph.  Rows are 16-byte aligned: base pointers and row strides (given
  * in elements) are multiples of 16 bytes, head h of a row starts head_dim * h further
- * on.  head_dim is 64 or 128; q_heads is a multiple of kv_heads.
+ * on.  head_dim is 64 or 128; q_heads is a multiple of kv_heads; scale is positive.
  *
  * Indices that live in device memory (positions, slots, page tables, lengths, sequence
  * bounds) are checked by the kernels: one that points outside its buffer is never
