@@ -11,16 +11,14 @@
 // moves from accumulator to operand layout with two movmatrix.  tcgen05 would
 // want 128 rows for 8 used ones, and the tensor pipe is idle either way.
 //
-// Work split.  The cache of all (sequence, key/value head) pairs is one long line
-// of 64-key units, cut into equal parts, one per SM, whatever the lengths are (read
-// on the device, so a captured graph follows them).  A part may end inside a pair:
-// its partial (o, m, l) then goes to the workspace and the last CTA of the pair to
-// arrive joins the parts in order, so results do not depend on timing.
-//
-// In a CTA, 8 warps take the segment's steps in turn, each with a ring of its own
-// (3 stages of 8 KB of keys and values, TMA boxes of 16 rows, page numbers looked
-// up one batch ahead): nothing but the join at a segment's end synchronises them,
-// and the rings run on across segments.
+// Work split.  The caches of all (sequence, key/value head) pairs ("items") form one long
+// line of steps (8 KB of keys and values each), cut into equal parts, one per warp, whatever the
+// lengths are (read on the device, so a captured graph follows them).  A warp runs through its
+// part alone: its own ring of TMA stages, its own running softmax, an item that lies whole in it
+// written out at once, so short caches cost no barrier.  An item cut between warps leaves
+// partial (o, m, l) in shared memory, joined at the block's end; one cut between blocks leaves
+// a partial in the workspace, and the last block of the item to arrive joins them.  Both joins
+// go in order along the line, so results do not depend on timing.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -32,12 +30,14 @@ namespace cz {
 namespace {
 
 constexpr int kWarps = 8;
-constexpr int kStages = 3;
+// 128 KB in flight per SM reach the card's rate; a third stage only lengthens the queue that the
+// last blocks wait in (128 x 4,000 tokens: 171 us with 3, 163 us with 2).
+constexpr int kStages = 2;
 constexpr int kStageBytes = 8192;  // keys, then values, of one step
-constexpr int kUnit = 64;          // keys per unit of the work split
-// A CTA takes at least this many units where that leaves CTAs idle: below 256 keys the
-// join over the workspace costs more than the shorter loop gains.
-constexpr int kMinUnits = 4;
+// With little work, an item of up to this many steps per warp stays in one block: the join over the
+// workspace costs more than the shorter loop gains.
+constexpr int kShort = 4;
+constexpr uint32_t kItemSteps = 2;  // what starting and ending an item costs a warp, in steps
 constexpr int kMaxTiles = 2;       // 8-head column tiles per pass
 constexpr int kSlotFloats = kMaxTiles * 8 * 128 + kMaxTiles * 8 * 2;  // o, then (m, l) per head
 
@@ -46,7 +46,8 @@ struct DecodeArgs {
     AttnDecodeParams p;
     uint32_t group, tiles;   // query heads per kv head; passes of NT * 8 of them
     float* slots;            // workspace: [grid][2][kSlotFloats]
-    uint32_t* counters;      // workspace: [grid] arrivals at the pair that begins in this CTA and goes on
+    uint32_t* counters;      // workspace: [grid] arrivals at the item that begins in this block and goes on
+    int box;                 // rows per TMA box: a step's, or 16 where pages are smaller or cut it
 };
 
 __device__ __forceinline__ float ex2(float x) {
@@ -55,12 +56,11 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 
-__device__ __forceinline__ void tma4d(uint32_t dst, const CUtensorMap* m, int x, int row, int head, int page,
-                                      uint64_t* bar) {
+__device__ __forceinline__ void tma5d(uint32_t dst, const CUtensorMap* m, int row, int head, int page, uint64_t* bar) {
     asm volatile(
-        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, "
-        "%5}], [%6];" ::"r"(dst),
-        "l"(reinterpret_cast<uint64_t>(m)), "r"(x), "r"(row), "r"(head), "r"(page), "r"(smem_u32(bar))
+        "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, "
+        "%5, %6}], [%7];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(m)), "r"(0), "r"(row), "r"(0), "r"(head), "r"(page), "r"(smem_u32(bar))
         : "memory");
 }
 
@@ -100,6 +100,11 @@ __device__ __forceinline__ uint32_t cvt_e4m3x2(uint32_t two) {
     asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"((uint16_t)two));
     return h;
 }
+__device__ __forceinline__ uint32_t atom_add_acq_rel(uint32_t* p, uint32_t v) {
+    uint32_t r;
+    asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], %2;" : "=r"(r) : "l"(p), "r"(v) : "memory");
+    return r;
+}
 template <bool F16>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
     uint32_t r;
@@ -116,43 +121,54 @@ __device__ __forceinline__ int seq_len(const AttnDecodeParams& p, int b) {
     const int most = (int)(p.table_width * p.kv.page_size);
     return n < 0 ? 0 : n > most ? most : n;
 }
-__device__ __forceinline__ uint32_t units_of(int n) { return (uint32_t)(n + kUnit - 1) / kUnit; }
 
-// Walks this CTA's part [pos, end) of the line.  The line holds, sequence by sequence,
-// `items` stretches (kv heads x passes) of units_of(len) units each, rounded up to
-// whole kMinUnits when `pad`.
+// The line: sequence by sequence, `items` stretches (kv heads x passes) of length() steps.
+struct Line {
+    int items;
+    uint32_t quota;  // steps per warp
+    bool whole;      // little work: items start on block boundaries
+
+    __device__ __forceinline__ uint32_t length(uint32_t n) const {
+        return n == 0 ? 0 : whole ? (n + kWarps * quota - 1) / (kWarps * quota) * (kWarps * quota) : n + kItemSteps;
+    }
+};
+
+// Walks a warp's part [pos, end) of the line.
+template <int TS>
 struct Walk {
-    uint32_t pos, end, off;  // place on the line; units of the current item before it
+    uint32_t pos, end, off;  // place on the line; steps of the current item before it
     int b, item, len;
-    uint32_t n, npad;
+    uint32_t n, room;        // steps of an item of b; what they take on the line
 
-    __device__ void enter(const AttnDecodeParams& p, int bb, bool pad) {
+    __device__ __forceinline__ void enter(const AttnDecodeParams& p, const Line& line, int bb) {
+#pragma unroll 1
         for (b = bb; b < p.B; ++b) {
             len = seq_len(p, b);
             if (len > 0) break;
         }
-        n = b < p.B ? units_of(len) : 0;
-        npad = pad ? (n + kMinUnits - 1) / kMinUnits * kMinUnits : n;
+        n = b < p.B ? (uint32_t)(len + TS - 1) / TS : 0;
+        room = line.length(n);
     }
-    // The next stretch with keys in it: tokens [t0, t1) of (b, item).  start = the item's own
-    // place on the line.  False at the part's end.
-    __device__ bool next(const AttnDecodeParams& p, int items, bool pad, int& sb, int& sitem, int& t0, int& t1,
-                         uint32_t& start, uint32_t& sn) {
+    // The next segment: keys [t0, t1) of (b, item), whose stretch begins at `start` on the line.
+    // False at the part's end.
+    __device__ __forceinline__ bool next(const AttnDecodeParams& p, const Line& line, int& sb, int& sitem, int& t0,
+                                         int& t1, int& slen, uint32_t& start) {
+#pragma unroll 1
         while (pos < end && b < p.B) {
-            const uint32_t u0 = off, take = min(npad - off, end - pos), u1 = min(u0 + take, n);
+            const uint32_t u0 = off, take = min(room - off, end - pos), u1 = min(u0 + take, n);
             sb = b;
             sitem = item;
-            t0 = (int)(u0 * kUnit);
-            t1 = min(len, (int)(u1 * kUnit));
+            slen = len;
+            t0 = (int)(u0 * TS);
+            t1 = min(len, (int)(u1 * TS));
             start = pos - u0;
-            sn = n;
             pos += take;
             off += take;
-            if (off == npad) {
+            if (off == room) {
                 off = 0;
-                if (++item == items) {
+                if (++item == line.items) {
                     item = 0;
-                    enter(p, b + 1, pad);
+                    enter(p, line, b + 1);
                 }
             }
             if (u1 > u0) return true;
@@ -168,10 +184,11 @@ struct Cfg {
     static constexpr int NBX = ROWB / BOXB;
     static constexpr int TS = kStageBytes / 2 / ROWB;  // keys per step
     static constexpr int NSUB = TS / 16;
-    static constexpr int BOX = 16 * BOXB;
     static constexpr int JROW = D + 4;
     static constexpr int RING = kWarps * kStages * kStageBytes;
-    static constexpr int JOIN = kWarps * 8 * JROW * 4;
+    // a warp's partial of the item it starts in; that of the item it ends in goes into its ring
+    static constexpr int PART = NT * 8 * JROW * 4;
+    static_assert(PART <= kStages * kStageBytes, "a partial fits the ring");
 };
 
 // Byte offset of 16-byte chunk c of row r (0..15) in a sub-tile: boxes of 16 rows, TMA's
@@ -189,18 +206,24 @@ __global__ void __launch_bounds__(kWarps * 32, 1) attn_decode_kernel(const __gri
     const AttnDecodeParams& p = A.p;
     extern __shared__ uint8_t raw[];
     uint8_t* base = raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u);
-    float* join = reinterpret_cast<float*>(base + C::RING);           // [warp][8][JROW]; the prologue's prefix before
-    float* stat = join + kWarps * 8 * C::JROW;                        // [warp][8][2]
+    uint32_t* prefix = reinterpret_cast<uint32_t*>(base + C::RING);  // prologue: places before each sequence (one item's)
     __shared__ uint64_t full[kWarps][kStages];
-    __shared__ uint32_t scan[kWarps + 1];
+    __shared__ uint32_t scan[kWarps][6];
+    // partials of the items a warp starts in (0) and ends in (1): item (-1: none), first and last of its keys here
+    struct Rec {
+        int item, b, begins, ends;
+        uint32_t start, steps;
+    };
+    __shared__ Rec recs[kWarps][2];
+    __shared__ float2 stat[kWarps][2][NT * 8];  // (m, l)
     __shared__ int abort_flag, never;
     __shared__ uint32_t last_flag;
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int g = lane >> 2, t4 = lane & 3;
-    const int items = (int)(p.kv.kv_heads * A.tiles);
 
     if (tid == 0) abort_flag = never = 0;
+    if (lane < 2) recs[warp][lane].item = -1;
     if (lane == 0) {
 #pragma unroll
         for (int s = 0; s < kStages; ++s) mbar_init(&full[warp][s], 1);
@@ -211,149 +234,203 @@ __global__ void __launch_bounds__(kWarps * 32, 1) attn_decode_kernel(const __gri
         prefetch_tensormap(&A.vmap);
     }
 
-    // ---- this CTA's part of the line ----
-    uint32_t* prefix = reinterpret_cast<uint32_t*>(join);  // units before each sequence (one item's)
-    uint32_t total = 0;
-    bool pad = false;
-    for (int round = 0; round < 2; ++round) {
-        const int per = (p.B + kWarps * 32 - 1) / (kWarps * 32);
-        uint32_t mine = 0;
-        for (int i = 0; i < per; ++i) {
-            const int b = tid * per + i;
-            if (b >= p.B) break;
-            const int n = seq_len(p, b);
-            if (round == 0 && blockIdx.x == 0 && __ldg(p.lens + b) != n) atomicOr(p.err, kAttnErrIndex);
-            const uint32_t u = units_of(n);
-            mine += pad ? (u + kMinUnits - 1) / kMinUnits * kMinUnits : u;
-        }
-        uint32_t inc = mine;
+    // ---- the line and this warp's part of it ----
+    // of the sequences: steps and item costs; blocks with 1, 2 and 4 steps a warp; the longest
+    Line line;
+    line.items = (int)(p.kv.kv_heads * A.tiles);
+    const uint32_t grid = gridDim.x, items = (uint32_t)line.items;
+    uint32_t sum[5] = {0, 0, 0, 0, 0};
+    auto count = [&](int b) {
+        const int l = seq_len(p, b);
+        if (blockIdx.x == 0 && warp == 0 && __ldg(p.lens + b) != l) atomicOr(p.err, kAttnErrIndex);
+        const uint32_t n = (uint32_t)(l + C::TS - 1) / C::TS;
+        sum[0] += n ? n + kItemSteps : 0;
+        sum[1] += (n + kWarps - 1) / kWarps;
+        sum[2] += (n + 2 * kWarps - 1) / (2 * kWarps);
+        sum[3] += (n + 4 * kWarps - 1) / (4 * kWarps);
+        sum[4] = max(sum[4], n);
+        return n;
+    };
+    auto decide = [&]() {
+        // little work (every item gets blocks of its own): the shortest loops that the blocks allow, but
+        // short items in one block
+        line.whole = sum[3] * items <= grid;
+        line.quota = !line.whole                 ? (sum[0] * items + grid * kWarps - 1) / (grid * kWarps)
+                     : sum[4] <= kShort * kWarps ? max(1u, (sum[4] + kWarps - 1) / kWarps)
+                     : sum[1] * items <= grid    ? 1
+                     : sum[2] * items <= grid    ? 2
+                                                 : 4;
+    };
+    auto reduce = [&]() {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sum[i] = __reduce_add_sync(0xffffffffu, sum[i]);
+        sum[4] = __reduce_max_sync(0xffffffffu, sum[4]);
+    };
+    auto scan32 = [&](uint32_t v) {  // inclusive sums over the lanes
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const uint32_t v = __shfl_up_sync(0xffffffffu, inc, o);
-            if (lane >= o) inc += v;
+            const uint32_t u = __shfl_up_sync(0xffffffffu, v, o);
+            if (lane >= o) v += u;
         }
+        return v;
+    };
+    uint32_t total, begin;  // begin: where the line's sequence `lo` starts
+    uint32_t bquota;        // a block's part
+    int lo = 0;             // the last sequence that begins at or before this warp's part (empty ones are skipped later)
+    if (p.B <= 32) {        // every warp for itself
+        const uint32_t n = lane < p.B ? count(lane) : 0;
+        reduce();
+        decide();
+        bquota = line.quota * kWarps;
+        const uint32_t mine = line.length(n), inc = scan32(mine);
+        total = __shfl_sync(0xffffffffu, inc, 31) * items;
+        const uint32_t pos = min(total, blockIdx.x * bquota + warp * line.quota);
+        const unsigned at = __ballot_sync(0xffffffffu, lane < p.B && (inc - mine) * items <= pos);
+        lo = 31 - __clz(at);
+        begin = __shfl_sync(0xffffffffu, inc - mine, lo) * items;
+    } else {
+        const int per = (p.B + kWarps * 32 - 1) / (kWarps * 32);
+#pragma unroll 1
+        for (int i = 0; i < per; ++i)
+            if (tid * per + i < p.B) count(tid * per + i);
+        reduce();
+        if (lane < 5)
+            scan[warp][lane] = lane == 0 ? sum[0] : lane == 1 ? sum[1] : lane == 2 ? sum[2] : lane == 3 ? sum[3] : sum[4];
         __syncthreads();
-        if (lane == 31) scan[warp] = inc;
+#pragma unroll
+        for (int i = 0; i < 5; ++i) sum[i] = lane < kWarps ? scan[lane][i] : 0;
+        reduce();
+        decide();
+        bquota = line.quota * kWarps;
+        uint32_t mine = 0;
+#pragma unroll 1
+        for (int i = 0; i < per; ++i) {
+            const int b = tid * per + i;
+            if (b < p.B) mine += line.length((uint32_t)(seq_len(p, b) + C::TS - 1) / C::TS);
+        }
+        const uint32_t inc = scan32(mine);
+        if (lane == 31) scan[warp][5] = inc;
         __syncthreads();
-        uint32_t before = inc - mine;
+        uint32_t place = inc - mine;
         total = 0;
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) {
-            if (w < warp) before += scan[w];
-            total += scan[w];
+            const uint32_t v = scan[w][5];
+            if (w < warp) place += v;
+            total += v;
         }
+        total *= items;
+#pragma unroll 1
         for (int i = 0; i < per; ++i) {
             const int b = tid * per + i;
             if (b >= p.B) break;
-            prefix[b] = before;
-            const uint32_t u = units_of(seq_len(p, b));
-            before += pad ? (u + kMinUnits - 1) / kMinUnits * kMinUnits : u;
+            prefix[b] = place;
+            place += line.length((uint32_t)(seq_len(p, b) + C::TS - 1) / C::TS);
         }
-        total *= items;
-        if (pad || (total + gridDim.x - 1) / gridDim.x >= kMinUnits) break;
-        pad = true;  // little work: whole kMinUnits per item, so that short caches are not split
-    }
-    __syncthreads();
-    const uint32_t quota = max((uint32_t)kMinUnits, (total + gridDim.x - 1) / gridDim.x);
-    // a sequence with nothing cached: zeros
-    for (int b = blockIdx.x; b < p.B; b += gridDim.x) {
-        if (seq_len(p, b) != 0) continue;
-        uint4* o = reinterpret_cast<uint4*>(p.out + (uint64_t)b * p.q_heads * D);
-        for (uint32_t i = tid; i < p.q_heads * D / 8; i += kWarps * 32) o[i] = make_uint4(0u, 0u, 0u, 0u);
-    }
-    Walk w0;
-    w0.pos = blockIdx.x * quota;
-    w0.end = min(total, w0.pos + quota);
-    if (w0.pos >= total) return;
-    {
-        int lo = 0, hi = p.B;  // the last sequence that begins at or before pos (empty ones are skipped by enter)
+        __syncthreads();
+        const uint32_t pos = min(total, blockIdx.x * bquota + warp * line.quota);
+        int hi = p.B;
+#pragma unroll 1
         while (hi - lo > 1) {
             const int mid = (lo + hi) / 2;
-            if (prefix[mid] * items <= w0.pos) lo = mid;
+            if (prefix[mid] * items <= pos) lo = mid;
             else hi = mid;
         }
-        w0.enter(p, lo, pad);
-        const uint32_t in = w0.pos - prefix[lo] * items;
-        w0.item = (int)(in / w0.npad);
-        w0.off = in % w0.npad;
+        begin = prefix[lo] * items;
+        __syncthreads();  // the prefix's room becomes the partials'
     }
-    __syncthreads();  // the prefix's room becomes the join's
+    // a sequence with nothing cached: zeros
+#pragma unroll 1
+    for (int b = blockIdx.x; b < p.B; b += grid) {
+        if (seq_len(p, b) != 0) continue;
+        uint4* o = reinterpret_cast<uint4*>(p.out + (uint64_t)b * p.q_heads * D);
+#pragma unroll 1
+        for (uint32_t i = tid; i < p.q_heads * D / 8; i += kWarps * 32) o[i] = make_uint4(0u, 0u, 0u, 0u);
+    }
+    if (blockIdx.x * bquota >= total) return;
+    Walk<C::TS> wc;
+    wc.pos = min(total, blockIdx.x * bquota + warp * line.quota);
+    wc.end = min(total, wc.pos + line.quota);
+    wc.b = p.B;
+    wc.off = 0;
+    wc.item = 0;
+    if (wc.pos < total) {
+        wc.enter(p, line, lo);
+        const uint32_t in = wc.pos - begin;
+        wc.item = (int)(in / wc.room);
+        wc.off = in % wc.room;
+    }
 
     // ---- producer side: batches of this warp's steps, page numbers one batch ahead ----
     constexpr int SPB = 32 / C::NSUB;  // steps per batch: a lane looks up one 16-key sub-tile
     struct Batch {
-        int kh, tok, t1, steps, page;  // first key, segment end, steps, this lane's page
+        int kh, tok, t1, steps, page, row;  // first key, segment end, steps, this lane's page and row in it
     };
-    Walk wp = w0;
-    int pb = 0, pitem = 0, pt0 = 0, pt1 = 0;  // the producer's segment and what is left of it
+    Walk<C::TS> wp = wc;
+    int pb = 0, pitem = 0, pt0 = 0, pt1 = 0;  // the producer's segment: what is left of it
     bool pmore = true;
-    auto fetch = [&](Batch& x) {
-        uint32_t st, sn;
-        x.steps = 0;
-        while (pmore) {
-            const int first = pt0 + warp * C::TS;
-            if (first < pt1) {
-                x.kh = pitem / (int)A.tiles;
-                x.tok = first;
-                x.t1 = pt1;
-                x.steps = min(SPB, (pt1 - first + kWarps * C::TS - 1) / (kWarps * C::TS));
-                const int tk = first + (lane / C::NSUB) * (kWarps * C::TS) + (lane % C::NSUB) * 16;
-                x.page = tk < pt1 ? __ldg(p.table + (uint64_t)pb * p.table_stride + (uint32_t)tk / p.kv.page_size) : 0;
-                pt0 += SPB * kWarps * C::TS;
-                return;
-            }
-            pmore = wp.next(p, items, pad, pb, pitem, pt0, pt1, st, sn);
-        }
-    };
     Batch cur, nxt;
-    cur.steps = 0;
-    fetch(nxt);
+    cur.steps = nxt.steps = 0;
     int bstep = 0, pstage = 0;
     uint8_t* ring = base + warp * kStages * kStageBytes;
+    // One step's copies.  (Called from one place, like both Walk::next: the code of an item's whole round
+    // has to stay in the instruction caches.)
     auto produce = [&]() {
-        if (bstep == cur.steps) {
+#pragma unroll 1
+        while (bstep == cur.steps && (pmore || nxt.steps)) {
             cur = nxt;
             bstep = 0;
-            if (cur.steps == 0) return;
-            fetch(nxt);
+            nxt.steps = 0;
+            if (pt0 >= pt1) {
+                int len;
+                uint32_t st;
+                pmore = wp.next(p, line, pb, pitem, pt0, pt1, len, st);
+            }
+            if (pmore) {
+                nxt.kh = pitem / (int)A.tiles;
+                nxt.tok = pt0;
+                nxt.t1 = pt1;
+                nxt.steps = min(SPB, (pt1 - pt0 + C::TS - 1) / C::TS);
+                const uint32_t tk = pt0 + lane * 16;
+                const uint32_t idx = tk / p.kv.page_size;
+                nxt.row = (int)(tk - idx * p.kv.page_size);
+                nxt.page = (int)tk < pt1 ? __ldg(p.table + (uint64_t)pb * p.table_stride + idx) : 0;
+                pt0 += SPB * C::TS;
+            }
         }
-        const int tok = cur.tok + bstep * (kWarps * C::TS);
+        if (bstep == cur.steps) return;
+        const int tok = cur.tok + bstep * C::TS;
         const int subs = min(C::NSUB, (cur.t1 - tok + 15) / 16);
         uint64_t* bar = &full[warp][pstage];
         const uint32_t dst = smem_u32(ring + pstage * kStageBytes);
-        if (lane == 0) mbar_arrive_expect_tx(bar, subs * 16 * C::ROWB * 2);
-#pragma unroll
-        for (int s = 0; s < C::NSUB; ++s) {
+        const int skip = A.box / 16;  // sub-tiles per box
+        if (lane == 0) mbar_arrive_expect_tx(bar, (subs + skip - 1) / skip * skip * 16 * C::ROWB * 2);
+#pragma unroll 1
+        for (int s = 0; s < subs; s += skip) {
             int page = __shfl_sync(0xffffffffu, cur.page, bstep * C::NSUB + s);
-            if (lane == 0 && s < subs) {
+            const int row = __shfl_sync(0xffffffffu, cur.row, bstep * C::NSUB + s);
+            if (lane == 0) {
                 if ((uint32_t)page >= p.kv.pages) {  // not followed
                     atomicOr(p.err, kAttnErrIndex);
                     page = 0;
                 }
-                const int row = (int)((uint32_t)(tok + s * 16) % p.kv.page_size);
-#pragma unroll
-                for (int x = 0; x < C::NBX; ++x) {
-                    const uint32_t d = dst + s * 16 * C::ROWB + x * C::BOX;
-                    const int col = x * C::BOXB / (F8 ? 1 : 2);
-                    tma4d(d, &A.kmap, col, row, cur.kh, page, bar);
-                    tma4d(d + kStageBytes / 2, &A.vmap, col, row, cur.kh, page, bar);
-                }
+                tma5d(dst + s * 16 * C::ROWB, &A.kmap, row, cur.kh, page, bar);
+                tma5d(dst + s * 16 * C::ROWB + kStageBytes / 2, &A.vmap, row, cur.kh, page, bar);
             }
         }
         ++bstep;
         pstage = pstage + 1 == kStages ? 0 : pstage + 1;
     };
+    int credit = kStages;  // stages free to fill
     __syncwarp();
-#pragma unroll
-    for (int s = 0; s < kStages; ++s) produce();
 
     // ---- consumer side ----
-    Walk wc = w0;
     int cstage = 0;
     uint32_t cphase = 0;
-    int b, item, t0, t1;
-    uint32_t start, units;
-    while (wc.next(p, items, pad, b, item, t0, t1, start, units)) {
+    int b, item, t0, t1, len;
+    uint32_t start;
+#pragma unroll 1
+    while (wc.next(p, line, b, item, t0, t1, len, start)) {
         const int kh = item / (int)A.tiles, head0 = (item % (int)A.tiles) * NT * 8;
         const int heads = min(NT * 8, (int)A.group - head0);  // of this pass
         const uint64_t hbase = (uint64_t)kh * A.group + head0;
@@ -417,7 +494,11 @@ __global__ void __launch_bounds__(kWarps * 32, 1) attn_decode_kernel(const __gri
             l[n][0] = l[n][1] = 0.f;
         }
 
-        for (int tok = t0 + warp * C::TS; tok < t1; tok += kWarps * C::TS) {
+#pragma unroll 1
+        for (int tok = t0;; tok += C::TS) {
+#pragma unroll 1
+            for (; credit > 0; --credit) produce();
+            if (tok >= t1) break;
             uint64_t* bar = &full[warp][cstage];
             if (!mbar_wait_bounded(bar, cphase, &abort_flag)) {
                 // reported, and carried on with what is there: every warp keeps its place in the joins
@@ -431,6 +512,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) attn_decode_kernel(const __gri
                 // rows of the last sub-tile past the end may hold anything, NaN included: their weights are 0,
                 // but 0 * NaN is not
                 uint8_t* vs = ring + cstage * kStageBytes + kStageBytes / 2 + (valid >> 4) * 16 * C::ROWB;
+#pragma unroll 1
                 for (int i = lane; i < (16 - (valid & 15)) * C::NBX * (C::BOXB / 16); i += 32) {
                     const int r = (valid & 15) + i / (C::NBX * (C::BOXB / 16)), c = i % (C::NBX * (C::BOXB / 16));
                     *reinterpret_cast<uint4*>(vs + chunk_at<C::BOXB>(r, c)) = make_uint4(0u, 0u, 0u, 0u);
@@ -560,127 +642,200 @@ __global__ void __launch_bounds__(kWarps * 32, 1) attn_decode_kernel(const __gri
             }
             __syncwarp();
             if (++cstage == kStages) cstage = 0, cphase ^= 1;
-            produce();
+            ++credit;
         }
 
-        // ---- the segment's warps joined; out, or a partial result for the pair's last CTA ----
-        const uint32_t c0 = start / quota, c1 = (start + units - 1) / quota;
-        const bool whole = c0 == c1;
-        float* slot = A.slots + ((uint64_t)blockIdx.x * 2 + (blockIdx.x == c0 ? 1 : 0)) * kSlotFloats;
-        const float vscale = p.kv.v_scale ? __ldg(p.kv.v_scale + kh) : 1.f;
-        constexpr int EPT = 8 * D / (kWarps * 32);  // output elements per thread: 4 or 2
-        const int jh = tid * EPT / D, jd = tid * EPT % D;
+        // ---- the segment's end ----
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            if (n * 8 >= heads) break;
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int d = 4; d < 32; d <<= 1) {
                 l[n][0] += __shfl_xor_sync(0xffffffffu, l[n][0], d);
                 l[n][1] += __shfl_xor_sync(0xffffffffu, l[n][1], d);
             }
-            float* jw = join + warp * 8 * C::JROW;
+        if (t0 == 0 && t1 == len) {  // the whole item: out
+            const float vscale = p.kv.v_scale ? __ldg(p.kv.v_scale + kh) : 1.f;
+            uint16_t* out = p.out + ((uint64_t)b * p.q_heads + hbase) * D;
 #pragma unroll
-            for (int k = 0; k < KS; ++k)
+            for (int n = 0; n < NT; ++n) {
+                const float r0 = l[n][0] > 0.f || l[n][0] != l[n][0] ? vscale / l[n][0] : 0.f;
+                const float r1 = l[n][1] > 0.f || l[n][1] != l[n][1] ? vscale / l[n][1] : 0.f;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int d = F8 ? k * 16 + 2 * g + (i >> 1) : k * 16 + g + (i >> 1) * 8;
-                    jw[(2 * t4 + (i & 1)) * C::JROW + d] = o[n][k][i];
-                }
-            if (g == 0) {
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    stat[(warp * 8 + 2 * t4 + i) * 2] = m[n][i];
-                    stat[(warp * 8 + 2 * t4 + i) * 2 + 1] = l[n][i];
+                for (int k = 0; k < KS; ++k) {
+                    const float* c = o[n][k];
+                    if (F8) {  // dims 16 k + 2 g, + 1 of heads 2 t4 and 2 t4 + 1
+                        const int h = n * 8 + 2 * t4;
+                        uint16_t* d = out + (uint64_t)h * D + k * 16 + 2 * g;
+                        if (h < heads) *reinterpret_cast<uint32_t*>(d) = pack2<false>(c[0] * r0, c[2] * r0);
+                        if (h + 1 < heads) *reinterpret_cast<uint32_t*>(d + D) = pack2<false>(c[1] * r1, c[3] * r1);
+                    } else {  // two heads of a dim -> two dims of a head
+                        const uint32_t lo = movm(pack2<false>(c[0] * r0, c[1] * r1));
+                        const uint32_t hi = movm(pack2<false>(c[2] * r0, c[3] * r1));
+                        uint16_t* d = out + (uint64_t)(n * 8 + g) * D + k * 16 + 2 * t4;
+                        if (n * 8 + g < heads) {
+                            *reinterpret_cast<uint32_t*>(d) = lo;
+                            *reinterpret_cast<uint32_t*>(d + 8) = hi;
+                        }
+                    }
                 }
             }
-            __syncthreads();
-            float mm = -INFINITY;
+        } else {
+            const int which = t0 == 0;  // an item begun here is the part's last: the ring is free for it
+            float* jw = reinterpret_cast<float*>(which ? ring : base + C::RING + warp * C::PART);
 #pragma unroll
-            for (int w = 0; w < kWarps; ++w) mm = fmaxf(mm, stat[(w * 8 + jh) * 2]);
-            const float zz = mm == -INFINITY ? 0.f : mm;
-            float acc[EPT], ll = 0.f;
+            for (int n = 0; n < NT; ++n) {
+#pragma unroll
+                for (int k = 0; k < KS; ++k)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int d = F8 ? k * 16 + 2 * g + (i >> 1) : k * 16 + g + (i >> 1) * 8;
+                        jw[(n * 8 + 2 * t4 + (i & 1)) * C::JROW + d] = o[n][k][i];
+                    }
+                if (g == 0) {
+#pragma unroll
+                    for (int i = 0; i < 2; ++i)
+                        stat[warp][which][n * 8 + 2 * t4 + i] = make_float2(m[n][i], l[n][i]);
+                }
+            }
+            if (lane == 0)
+                recs[warp][which] = Rec{item, b, t0 == 0, t1 == len, start, (uint32_t)(len + C::TS - 1) / C::TS};
+        }
+    }
+
+    // ---- items cut between this block's warps, or between blocks ----
+    __syncthreads();
+    constexpr int EPT = D / 32;  // a warp a head, 4 or 2 dims a lane
+    const int jh = warp, jd = lane * EPT;
+    auto finish = [&](const Rec& r, int n, float* acc, float ll) {
+        const int kh = r.item / (int)A.tiles, h = (r.item % (int)A.tiles) * NT * 8 + n * 8 + jh;
+        if (h >= (int)A.group) return;
+        const float vscale = p.kv.v_scale ? __ldg(p.kv.v_scale + kh) : 1.f;
+        const float f = ll > 0.f || ll != ll ? vscale / ll : 0.f;
+        uint32_t* dst = reinterpret_cast<uint32_t*>(
+            p.out + ((uint64_t)r.b * p.q_heads + (uint64_t)kh * A.group + h) * D + jd);
+#pragma unroll
+        for (int i = 0; i < EPT; i += 2) dst[i / 2] = pack2<false>(acc[i] * f, acc[i + 1] * f);
+    };
+    // lane x looks after record x (warp x / 2, kind x % 2): an item's records follow one another, the
+    // first of them one that begins it, unless it came from the block before
+    const Rec& mine = recs[(lane >> 1) & 7][lane & 1];
+    const bool has = lane < 2 * kWarps && mine.item >= 0;
+    const uint32_t have = __ballot_sync(0xffffffffu, has), begs = __ballot_sync(0xffffffffu, has && mine.begins);
+    const uint32_t fins = __ballot_sync(0xffffffffu, has && mine.ends);
+    int open_left = -1, open_right = -1;  // first records of the items that go on in other blocks: before, or only after
+#pragma unroll 1
+    for (uint32_t left = have; left;) {
+        const int x = __ffs(left) - 1;
+        const uint32_t later = begs & left & ~(1u << x);
+        const uint32_t group = left & (later ? (later & (0u - later)) - 1 : 0xffffffffu);
+        left &= ~group;
+        const bool begins = begs >> x & 1, done = begins && (fins & group);
+        if (!done) (begins ? open_right : open_left) = x;
+        float* slot = A.slots + ((uint64_t)blockIdx.x * 2 + begins) * kSlotFloats;
+#pragma unroll 1
+        for (int n = 0; n < NT; ++n) {
+            const bool in = lane < 2 * kWarps && (group >> lane & 1);
+            const float2 ml = in ? stat[(lane >> 1) & 7][lane & 1][n * 8 + jh] : make_float2(-INFINITY, 0.f);
+            const float mm = warp_max(ml.x), zz = mm == -INFINITY ? 0.f : mm;
+            const float f = ex2(ml.x - zz), ll = warp_sum(f * ml.y);
+            float acc[EPT];
 #pragma unroll
             for (int i = 0; i < EPT; ++i) acc[i] = 0.f;
 #pragma unroll
-            for (int w = 0; w < kWarps; ++w) {
-                const float f = ex2(stat[(w * 8 + jh) * 2] - zz);
-                ll = __fmaf_rn(f, stat[(w * 8 + jh) * 2 + 1], ll);
+            for (int z = 0; z < 2 * kWarps; ++z) {
+                const float fz = __shfl_sync(0xffffffffu, f, z);
+                if (group >> z & 1) {
+                    const float* v = reinterpret_cast<const float*>(z & 1 ? base + (z >> 1) * kStages * kStageBytes
+                                                                          : base + C::RING + (z >> 1) * C::PART) +
+                                     (n * 8 + jh) * C::JROW + jd;
 #pragma unroll
-                for (int i = 0; i < EPT; ++i) acc[i] = __fmaf_rn(f, join[(w * 8 + jh) * C::JROW + jd + i], acc[i]);
-            }
-            if (whole) {
-                if (n * 8 + jh < heads) {
-                    const float r = ll > 0.f || ll != ll ? vscale / ll : 0.f;
-                    uint32_t* dst = reinterpret_cast<uint32_t*>(
-                        p.out + ((uint64_t)b * p.q_heads + hbase + n * 8 + jh) * D + jd);
-#pragma unroll
-                    for (int i = 0; i < EPT; i += 2) dst[i / 2] = pack2<false>(acc[i] * r, acc[i + 1] * r);
+                    for (int i = 0; i < EPT; ++i) acc[i] = __fmaf_rn(fz, v[i], acc[i]);
                 }
+            }
+            if (done) {
+                finish(recs[x >> 1][x & 1], n, acc, ll);
             } else {
 #pragma unroll
                 for (int i = 0; i < EPT; ++i) slot[(n * 8 + jh) * D + jd + i] = acc[i];
-                if (jd == 0) {
-                    slot[kMaxTiles * 8 * 128 + (n * 8 + jh) * 2] = mm;
-                    slot[kMaxTiles * 8 * 128 + (n * 8 + jh) * 2 + 1] = ll;
-                }
+                if (jd == 0) *(reinterpret_cast<float2*>(slot + kMaxTiles * 8 * 128) + n * 8 + jh) = make_float2(mm, ll);
             }
-            __syncthreads();  // the join's room is free again
         }
-        if (whole) continue;
-        __threadfence();
-        __syncthreads();
+    }
+#pragma unroll 1
+    for (int side = 0; side < 2; ++side) {
+        const int x = side ? open_right : open_left;
+        if (x < 0) continue;
+        const Rec& r = recs[x >> 1][x & 1];
+        const uint32_t c0 = r.start / bquota, c1 = (r.start + r.steps - 1) / bquota;
+        __syncthreads();  // the partial is written; then one release / acquire by thread 0
         if (tid == 0) {
-            const uint32_t before = atomicAdd(A.counters + c0, 1u);
-            last_flag = before == c1 - c0;
-            if (before == c1 - c0) A.counters[c0] = 0;  // as found, for the next call
+            const uint32_t arrived = atom_add_acq_rel(A.counters + c0, 1u);
+            last_flag = arrived == c1 - c0;
+            if (last_flag) A.counters[c0] = 0;  // as found, for the next call
         }
         __syncthreads();
         if (!last_flag) continue;
-        __threadfence();
-#pragma unroll
+        // the item's partials in order, a batch of loads in flight at a time (one at a time would cost a
+        // trip to L2 each)
+        constexpr int BATCH = 24;
+        const int parts = (int)(c1 - c0) + 1;
+#pragma unroll 1
         for (int n = 0; n < NT; ++n) {
             const int h = n * 8 + jh;
-            if (h >= heads) continue;
-            const uint64_t step = 2 * kSlotFloats;
-            const float* sl = A.slots + (uint64_t)c0 * step + kSlotFloats;  // the first CTA's second slot, then first slots
-            float mm = -INFINITY, ll = 0.f, acc[EPT];
+            float acc[EPT], mm = -INFINITY, ll = 0.f;
 #pragma unroll
             for (int i = 0; i < EPT; ++i) acc[i] = 0.f;
-            for (uint32_t c = c0; c <= c1; ++c) {
-                const float* x = c == c0 ? sl : A.slots + (uint64_t)c * step;
-                mm = fmaxf(mm, __ldcg(x + kMaxTiles * 8 * 128 + h * 2));
-            }
-            const float zz = mm == -INFINITY ? 0.f : mm;
-#pragma unroll 4
-            for (uint32_t c = c0; c <= c1; ++c) {
-                const float* x = c == c0 ? sl : A.slots + (uint64_t)c * step;
-                const float f = ex2(__ldcg(x + kMaxTiles * 8 * 128 + h * 2) - zz);
-                ll = __fmaf_rn(f, __ldcg(x + kMaxTiles * 8 * 128 + h * 2 + 1), ll);
+#pragma unroll 1
+            for (int c = 0; c < parts; c += BATCH) {
+                float2 ml[BATCH];
+                float v[BATCH][EPT];
 #pragma unroll
-                for (int i = 0; i < EPT; i += 2) {
-                    const float2 v = __ldcg(reinterpret_cast<const float2*>(x + h * D + jd + i));
-                    acc[i] = __fmaf_rn(f, v.x, acc[i]);
-                    acc[i + 1] = __fmaf_rn(f, v.y, acc[i + 1]);
+                for (int j = 0; j < BATCH; ++j) {
+                    const int q = min(c + j, parts - 1);
+                    const float* x = A.slots + ((uint64_t)(c0 + q) * 2 + (q == 0 ? 1 : 0)) * kSlotFloats;
+                    ml[j] = __ldcg(reinterpret_cast<const float2*>(x + kMaxTiles * 8 * 128) + h);
+                    if (EPT == 4) {
+                        const float4 w = __ldcg(reinterpret_cast<const float4*>(x + h * D + jd));
+                        v[j][0] = w.x, v[j][1] = w.y, v[j][EPT - 2] = w.z, v[j][EPT - 1] = w.w;
+                    } else {
+                        const float2 w = __ldcg(reinterpret_cast<const float2*>(x + h * D + jd));
+                        v[j][0] = w.x, v[j][1] = w.y;
+                    }
+                }
+                float top = mm;
+#pragma unroll
+                for (int j = 0; j < BATCH; ++j) top = fmaxf(top, c + j < parts ? ml[j].x : -INFINITY);
+                const float zz = top == -INFINITY ? 0.f : top, a = ex2(mm - zz);
+                mm = top;
+                ll *= a;
+#pragma unroll
+                for (int i = 0; i < EPT; ++i) acc[i] *= a;
+#pragma unroll
+                for (int j = 0; j < BATCH; ++j) {
+                    if (c + j < parts) {
+                        const float f = ex2(ml[j].x - zz);
+                        ll = __fmaf_rn(f, ml[j].y, ll);
+#pragma unroll
+                        for (int i = 0; i < EPT; ++i) acc[i] = __fmaf_rn(f, v[j][i], acc[i]);
+                    }
                 }
             }
-            const float r = ll > 0.f || ll != ll ? vscale / ll : 0.f;
-            uint32_t* dst = reinterpret_cast<uint32_t*>(p.out + ((uint64_t)b * p.q_heads + hbase + h) * D + jd);
-#pragma unroll
-            for (int i = 0; i < EPT; i += 2) dst[i / 2] = pack2<false>(acc[i] * r, acc[i + 1] * r);
+            finish(r, n, acc, ll);
         }
     }
 }
 
-// The cache as a tensor map of 16-row boxes.
-bool make_kv_map(CUtensorMap* map, const KvView& kv, const uint8_t* base, uint64_t page_stride) {
+// The cache as a tensor map: [page][head][128-byte column block][row][columns], boxes of `rows` rows
+// of all column blocks, each block's rows together in shared memory.
+bool make_kv_map(CUtensorMap* map, const KvView& kv, const uint8_t* base, uint64_t page_stride, uint32_t rows) {
     const EncodeTiled fn = encode_tiled();
     if (!fn) return false;
     const uint64_t elt = kv.e4m3 ? 1 : 2, rowb = kv.head_dim * elt, boxb = rowb < 128 ? rowb : 128;
-    const cuuint64_t dims[4] = {kv.head_dim, kv.page_size, kv.kv_heads, kv.pages};
-    const cuuint64_t strides[3] = {rowb, rowb * kv.page_size, page_stride * elt};
-    const cuuint32_t box[4] = {(cuuint32_t)(boxb / elt), 16, 1, 1};
-    const cuuint32_t one[4] = {1, 1, 1, 1};
-    return fn(map, kv.e4m3 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4,
+    const cuuint64_t dims[5] = {boxb / elt, kv.page_size, rowb / boxb, kv.kv_heads, kv.pages};
+    const cuuint64_t strides[4] = {rowb, boxb, rowb * kv.page_size, page_stride * elt};
+    const cuuint32_t box[5] = {(cuuint32_t)(boxb / elt), rows, (cuuint32_t)(rowb / boxb), 1, 1};
+    const cuuint32_t one[5] = {1, 1, 1, 1, 1};
+    return fn(map, kv.e4m3 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 5,
               const_cast<uint8_t*>(base), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
               boxb == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
@@ -689,11 +844,17 @@ bool make_kv_map(CUtensorMap* map, const KvView& kv, const uint8_t* base, uint64
 size_t counter_bytes(int num_sms) { return ((size_t)num_sms * 4 + 255) / 256 * 256; }
 
 template <int D, bool F8, int NT>
-int launch(const DecodeArgs& a, int grid, cudaStream_t st) {
+int launch(DecodeArgs& a, int grid, cudaStream_t st) {
     using C = Cfg<D, F8, NT>;
-    const size_t room = C::JOIN + kWarps * 8 * 2 * 4, prefix = (size_t)a.p.B * 4;
-    const size_t most = 1024 + C::RING + (room > 4 * 4096 ? room : 4 * 4096);
-    const size_t smem = 1024 + C::RING + (room > prefix ? room : prefix);
+    a.box = a.p.kv.page_size % C::TS == 0 ? C::TS : 16;
+    if (!make_kv_map(&a.kmap, a.p.kv, a.p.kv.k, a.p.kv.k_page, a.box) ||
+        !make_kv_map(&a.vmap, a.p.kv, a.p.kv.v, a.p.kv.v_page, a.box))
+        return CZ_ESHAPE;
+    // behind the rings, one after the other: the prefix [B], the partials
+    const size_t parts = kWarps * C::PART, prefix = (size_t)a.p.B * 4;
+    const size_t smem = 1024 + C::RING + (parts > prefix ? parts : prefix);
+    constexpr size_t most = 227 * 1024 - 4096;  // beside the static variables
+    if (smem > most) return CZ_ESHAPE;
     static bool set = false;  // the library's lock is held
     if (!set) {
         if (cudaFuncSetAttribute(attn_decode_kernel<D, F8, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
@@ -717,11 +878,9 @@ int attn_decode_launch(const AttnDecodeParams& p, int num_sms, cudaStream_t st) 
     a.group = p.q_heads / p.kv.kv_heads;
     const bool two = a.group > 8;
     a.tiles = two ? (a.group + 15) / 16 : 1;
-    // the split's line and its parts' ends are counted in 32 bits
-    const uint64_t units = ((uint64_t)p.table_width * p.kv.page_size + kUnit - 1) / kUnit + kMinUnits;
-    if ((uint64_t)p.B * p.kv.kv_heads * a.tiles * units >= 0x7fffffffu) return CZ_ESHAPE;
-    if (!make_kv_map(&a.kmap, p.kv, p.kv.k, p.kv.k_page) || !make_kv_map(&a.vmap, p.kv, p.kv.v, p.kv.v_page))
-        return CZ_ESHAPE;
+    // the line and its parts' ends are counted in 32 bits; a step is 16 keys or more
+    const uint64_t steps = (uint64_t)p.table_width * p.kv.page_size / 16 + kItemSteps + kWarps * kShort;
+    if ((uint64_t)p.B * p.kv.kv_heads * a.tiles * steps >= 0x7fff0000u) return CZ_ESHAPE;
     a.counters = reinterpret_cast<uint32_t*>(p.workspace);
     a.slots = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(p.workspace) + counter_bytes(num_sms));
     const bool d128 = p.kv.head_dim == 128;
