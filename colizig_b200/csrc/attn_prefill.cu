@@ -15,7 +15,7 @@
 // the tile (16 tokens of 8 heads), and the diagonal wastes at most 16 of 128 keys there.
 //
 // Warps: 0-3 and 4-7 softmax of query tile 0 and 1 (a thread a row), 8 TMA loads, 9 MMA
-// issue.  Blocks take tiles from the largest key count down, so the last to finish are short.
+// issue (10 and 11 lend their registers: 208 a thread for softmax, 88 for the rest).  Blocks take tiles from the largest key count down, so the last to finish are short.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -26,13 +26,17 @@
 namespace cz {
 namespace {
 
-constexpr int kThreads = 320;
+constexpr int kThreads = 384;
 constexpr int kKeys = 128;     // keys per tile
 constexpr uint32_t kTmemCols = 512;
 // A row's old maximum stays in use until a new one is more than this many powers of two
 // above it: P and l then grow to at most 2^8, far inside f32 and bf16, and most tiles
 // rescale nothing.  The result does not depend on it (o and l share the factor).
 constexpr float kSlack = 8.f;
+// Of every kPolyOf pairs of weights one is computed on the FMA pipe (exp2_pair), the rest by ex2: the
+// exponentials of two tiles would keep the special-function pipe as busy as the products keep the
+// tensor pipe.
+constexpr int kPolyOf = 4;
 
 struct PrefillArgs {
     CUtensorMap qmap, kmap, vmap;  // [rows][heads][D] in boxes of 64 columns
@@ -52,7 +56,7 @@ struct Cfg {
 };
 
 struct Bars {
-    uint64_t qfull[2], full[8], empty[8], sfull[2], pready[2], odone[2], drain;
+    uint64_t qfull[2], full[8], empty[8], sfull[2], pready[2][2], odone[2], vask, vclean, drain;
     uint32_t tmem;
     int abort, never;
     int q0, nq, k0, nk, tile;  // this block's sequence and query tile pair (tile < 0: none)
@@ -87,21 +91,28 @@ __host__ __device__ constexpr uint32_t idesc(int M, int N, bool bmn) {
     return (1u << 4) | (1u << 7) | (1u << 10) | (bmn ? 1u << 16 : 0u) | ((uint32_t)(N >> 3) << 17) |
            ((uint32_t)(M >> 4) << 24);
 }
+// The issuing warp runs converged and one elected lane issues: with warp-uniform operands the
+// descriptors stay in uniform registers (issued from a divergent branch, a product cost some 100 cycles
+// more than it took the tensor pipe).
 __device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t acc) {
     asm volatile(
-        "{\n.reg .pred p;\nsetp.ne.u32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d),
+        "{\n.reg .pred p, e;\nelect.sync _|e, 0xffffffff;\nsetp.ne.u32 p, %4, 0;\n"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d),
         "l"(a), "l"(b), "r"(id), "r"(acc)
         : "memory");
 }
 __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t id, uint32_t acc) {
     asm volatile(
-        "{\n.reg .pred p;\nsetp.ne.u32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(d),
+        "{\n.reg .pred p, e;\nelect.sync _|e, 0xffffffff;\nsetp.ne.u32 p, %4, 0;\n"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(d),
         "r"(a), "l"(b), "r"(id), "r"(acc)
         : "memory");
 }
 __device__ __forceinline__ void commit(uint64_t* bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
-                 : "memory");
+    asm volatile(
+        "{\n.reg .pred e;\nelect.sync _|e, 0xffffffff;\n"
+        "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}" ::"r"(smem_u32(bar))
+        : "memory");
 }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
@@ -119,14 +130,12 @@ __device__ __forceinline__ void ld32(uint32_t* r, uint32_t a) {
         : "r"(a)
         : "memory");
 }
-__device__ __forceinline__ void st32(uint32_t a, const uint32_t* r) {
+__device__ __forceinline__ void ld16(uint32_t* r, uint32_t a) {
     asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,"
-        "%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};" ::"r"(r[0]),
-        "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
-        "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]),
-        "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]),
-        "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(a)
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(a)
         : "memory");
 }
 __device__ __forceinline__ void st16(uint32_t a, const uint32_t* r) {
@@ -136,6 +145,55 @@ __device__ __forceinline__ void st16(uint32_t a, const uint32_t* r) {
         "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
         "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(a)
         : "memory");
+}
+typedef unsigned long long f2;  // two f32 in a register pair
+__device__ __forceinline__ f2 pair(float a, float b) {
+    f2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void unpair(f2 x, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(x)); }
+__device__ __forceinline__ f2 fma2(f2 a, f2 b, f2 c) {
+    f2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ f2 add2(f2 a, f2 b) {
+    f2 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+// Maximum of three, NaN if one is NaN.
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+// 2^t of two t <= 16 without the special-function pipe: t = n + f, n whole, |f| <= 1/2; 2^f by
+// the cubic of least largest relative error on that interval (Remez exchange, 7.5e-5, a
+// fiftieth of the rounding to bf16 that follows), n into the exponent.  t under -126 counts as -126.
+__device__ __forceinline__ void exp2_pair(f2 t, float& a, float& b) {
+    unpair(t, a, b);
+    const f2 x = pair(fmaxf(a, -126.f), fmaxf(b, -126.f));
+    const f2 u = add2(x, pair(12582912.f, 12582912.f));  // 1.5 * 2^23: n in the low bits
+    const f2 f = add2(x, fma2(u, pair(-1.f, -1.f), pair(12582912.f, 12582912.f)));
+    f2 y = fma2(pair(0.0551716685295105f, 0.0551716685295105f), f, pair(0.2426111251115799f, 0.2426111251115799f));
+    y = fma2(y, f, pair(0.6932609677314758f, 0.6932609677314758f));
+    y = fma2(y, f, pair(0.9999280571937561f, 0.9999280571937561f));
+    float ua, ub;
+    unpair(u, ua, ub);
+    unpair(y, a, b);
+    a = __uint_as_float(__float_as_uint(a) + (__float_as_uint(ua) << 23));
+    b = __uint_as_float(__float_as_uint(b) + (__float_as_uint(ub) << 23));
+}
+// A bounded wait without calls (setmaxnreg and calls do not go together).
+__device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, const volatile int* abort) {
+#pragma unroll 1
+    for (uint32_t it = 0; it < CZ_SPIN_LIMIT; ++it) {
+        if (mbar_try_wait(bar, parity)) return true;
+        if ((it & 15) == 15 && *abort) return false;
+    }
+    return false;
 }
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
     uint32_t r;
@@ -256,13 +314,16 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefill_kernel(const __grid_
         for (int i = 0; i < 2; ++i) {
             mbar_init(&B.qfull[i], 1);
             mbar_init(&B.sfull[i], 1);
-            mbar_init(&B.pready[i], 4);
+            mbar_init(&B.pready[i][0], 4);
+            mbar_init(&B.pready[i][1], 4);
             mbar_init(&B.odone[i], 1);
         }
         for (int i = 0; i < C::STAGES; ++i) {
             mbar_init(&B.full[i], 1);
             mbar_init(&B.empty[i], 1);
         }
+        mbar_init(&B.vask, 1);
+        mbar_init(&B.vclean, 1);
         mbar_init(&B.drain, 1);
         B.abort = B.never = 0;
         fence_mbarrier_init();
@@ -292,15 +353,20 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefill_kernel(const __grid_
         n[i] = tile < 0 || tok[i] >= nq || last < 0 ? 0 : last / kKeys + 1;
     }
     const int nmax = max(n[0], n[1]);
+    // keys of the last tile that belong to the sequence; products past them are left out, and the rows that
+    // fill up the last 16 (a neighbour's, of any value) are cleared first
+    const int last_keys = nmax > 0 ? min(kKeys, nk - (nmax - 1) * kKeys) : 0;
+    const bool unclean = last_keys & 15;
 
     auto gave_up = [&]() {
         *abort = 1;
         atomicOr(p.err, kAttnErrWait);
     };
 
-    if (tile < 0) {
-        // more blocks than query tiles (the grid is sized without reading the bounds)
-    } else if (warp == 8) {
+    // registers: 2 x 208 + 88 = 3 x 168, what the block was launched with
+    if (warp >= 8) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+      if (tile >= 0 && warp == 8) {
         // ---------------- loads ----------------
         if (lane == 0 && nmax > 0) {
             const uint32_t qbytes = (uint32_t)(A.tokens * A.pack) * 128 * C::NX;
@@ -316,7 +382,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefill_kernel(const __grid_
             auto load_kv = [&](const CUtensorMap* m, int j) {
                 const int s = issued % C::STAGES;
                 if (issued >= C::STAGES &&
-                    !mbar_wait_bounded(&B.empty[s], ((issued / C::STAGES) & 1) ^ 1, abort)) {
+                    !wait_bar(&B.empty[s], ((issued / C::STAGES) & 1) ^ 1, abort)) {
                     gave_up();
                     return false;
                 }
@@ -334,92 +400,114 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefill_kernel(const __grid_
             for (int j = 1; j < nmax && ok; ++j) ok = load_kv(&A.kmap, j) && load_kv(&A.vmap, j);
             // no copy stays in flight behind the block's end (all have landed unless a wait gave up)
             for (int i = max(0, issued - C::STAGES); i < issued; ++i)
-                if (!mbar_wait_bounded(&B.full[i % C::STAGES], (i / C::STAGES) & 1, &B.never)) gave_up();
+                if (!wait_bar(&B.full[i % C::STAGES], (i / C::STAGES) & 1, &B.never)) gave_up();
         }
         __syncwarp();
-    } else if (warp == 9) {
+      } else if (tile >= 0 && warp == 9) {
         // ---------------- MMA ----------------
         constexpr uint32_t IDS = idesc(128, kKeys, false), IDO = idesc(128, D, true);
+        const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+        const uint64_t dq = desc_k(smem_u32(sq)), dk = desc_k(smem_u32(skv));
+        const uint64_t dv = desc_mn(smem_u32(skv), kKeys * 128);
         auto wait = [&](uint64_t* bar, uint32_t parity) {
-            bool ok = true;
-            if (lane == 0) {
-                ok = mbar_wait_bounded(bar, parity, abort);
-                if (!ok) gave_up();
-            }
-            return (bool)__shfl_sync(0xffffffffu, ok, 0);
+            const bool ok = __all_sync(0xffffffffu, wait_bar(bar, parity, abort));
+            if (!ok) gave_up();
+            return ok;
         };
-        auto stage = [&](int use) { return skv + (use % C::STAGES) * C::KVBYTES; };
-        auto wait_kv = [&](int use) { return wait(&B.full[use % C::STAGES], (use / C::STAGES) & 1); };
-        auto qk = [&](int i, int j) {  // S_i = Q_i K_j^T
-            if (lane == 0) {
-                const uint32_t qa = smem_u32(sq + i * C::QBYTES), ka = smem_u32(stage(2 * j));
+        // the ring's uses in order: K_0, V_0, K_1, V_1, ...
+        int use = 0, ustage = 0;
+        uint32_t uphase = 0;
+        auto wait_kv = [&]() { return wait(&B.full[ustage], uphase); };
+        auto next_kv = [&]() {
+            const int st = ustage;
+            ++use;
+            if (++ustage == C::STAGES) ustage = 0, uphase ^= 1;
+            return st;
+        };
+        auto qk = [&](int i, int st) {  // S_i = Q_i K^T
 #pragma unroll
-                for (int k = 0; k < D / 16; ++k)
-                    mma_ss(tmem + i * 128, desc_k(qa + (k / 4) * 128 * 128) + (k % 4) * 2,
-                           desc_k(ka + (k / 4) * kKeys * 128) + (k % 4) * 2, IDS, k > 0);
-                commit(&B.sfull[i]);
+            for (int k = 0; k < D / 16; ++k) {
+                const uint32_t off = (k / 4) * (128 * 128 / 16) + (k % 4) * 2;
+                mma_ss(tm + i * 128, dq + (uint32_t)(i * C::QBYTES / 16 + off), dk + (uint32_t)(st * C::KVBYTES / 16 + off),
+                       IDS, k > 0);
             }
-            __syncwarp();
+            commit(&B.sfull[i]);
         };
-        auto done_kv = [&](int use) {
-            if (lane == 0) commit(&B.empty[use % C::STAGES]);
-            __syncwarp();
-        };
-        bool ok = nmax == 0 || wait_kv(0);
+        bool ok = nmax == 0 || wait_kv();
+        int kst = next_kv();
 #pragma unroll
         for (int i = 0; i < 2; ++i)
             if (ok && n[i] > 0) {
                 ok = wait(&B.qfull[i], 0);
-                if (ok) qk(i, 0);
+                if (ok) qk(i, kst);
             }
-        if (ok && nmax > 0) done_kv(0);
+        if (ok && nmax > 0) commit(&B.empty[kst]);
+#pragma unroll 1
         for (int j = 0; j < nmax && ok; ++j) {
-            // keys of this tile that belong to the sequence; products past them are left out, and the
-            // rows that fill up the last 16 (a neighbour's, of any value) are cleared
-            const int valid = min(kKeys, nk - j * kKeys), ksteps = (valid + 15) / 16;
-            ok = wait_kv(2 * j + 1);
-            if (!ok) break;
-            if (valid & 15) {
-                uint8_t* v = stage(2 * j + 1);
-                for (int i = lane; i < (ksteps * 16 - valid) * 8 * C::NX; i += 32) {
-                    const int r = valid + i / (8 * C::NX), c = i % (8 * C::NX);
-                    *reinterpret_cast<uint4*>(v + (c >> 3) * kKeys * 128 + r * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
-                }
-                fence_proxy_async_smem();
-                __syncwarp();
-            }
             const bool more = j + 1 < nmax;
-            if (more) {
-                ok = wait_kv(2 * j + 2);
-                if (!ok) break;
-            }
+            const int ksteps = more ? kKeys / 16 : (last_keys + 15) / 16;
+            ok = wait_kv();
+            if (!ok) break;
+            bool ask = unclean && !more;
+            if (ask && lane == 0) mbar_arrive(&B.vask);
+            __syncwarp();
+            const int vst = next_kv();
+            bool kwait = more;
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                if (j >= n[i]) continue;
-                ok = wait(&B.pready[i], j & 1);
-                if (!ok) break;
-                fence_after();
-                if (lane == 0) {
-                    const uint32_t va = smem_u32(stage(2 * j + 1));
-                    for (int k = 0; k < ksteps; ++k)
-                        mma_ts(tmem + C::OCOL + i * 128, tmem + i * 128 + k * 8, desc_mn(va + k * 2048, kKeys * 128),
+                if (j >= n[i] || !ok) continue;
+                auto pv = [&](int k) {
+                    if (k < ksteps)
+                        mma_ts(tm + C::OCOL + i * 128, tm + i * 128 + k * 8, dv + (uint32_t)((vst * C::KVBYTES + k * 2048) / 16),
                                IDO, j > 0 || k > 0);
-                    if (j + 1 == n[i]) commit(&B.odone[i]);
+                };
+                // the first 64 keys' products run under the other weights' exponentials
+                ok = wait(&B.pready[i][0], j & 1) && (!ask || wait(&B.vclean, 0));
+                if (!ok) continue;
+                ask = false;
+                fence_after();
+#pragma unroll
+                for (int k = 0; k < 4; ++k) pv(k);
+                ok = wait(&B.pready[i][1], j & 1);
+                if (!ok) continue;
+                fence_after();
+#pragma unroll
+                for (int k = 4; k < 8; ++k) pv(k);
+                if (j + 1 == n[i]) {
+                    commit(&B.odone[i]);
+                } else {
+                    if (kwait) {
+                        ok = wait_kv();
+                        kst = next_kv();
+                        kwait = false;
+                    }
+                    if (ok) qk(i, kst);  // into S_i: in order behind the product that reads P_i from it
                 }
-                __syncwarp();
-                if (j + 1 < n[i]) qk(i, j + 1);  // into S_i: in order behind the product that reads P_i from it
             }
             if (!ok) break;
-            done_kv(2 * j + 1);
-            if (more) done_kv(2 * j + 2);
+            commit(&B.empty[vst]);
+            if (more) commit(&B.empty[kst]);
         }
-        if (lane == 0) {  // every product has finished before TMEM is given back
-            commit(&B.drain);
-            if (!mbar_wait_bounded(&B.drain, 0, &B.never)) gave_up();
-        }
+        // every product has finished before TMEM is given back
+        commit(&B.drain);
+        if (!wait_bar(&B.drain, 0, &B.never)) gave_up();
         __syncwarp();
-    } else {
+      } else if (tile >= 0 && warp == 10 && unclean) {
+        // ---------------- the last values' tail ----------------
+        if (__all_sync(0xffffffffu, wait_bar(&B.vask, 0, abort))) {
+            uint8_t* v = skv + ((2 * nmax - 1) % C::STAGES) * C::KVBYTES;
+            for (int i = lane; i < (16 - (last_keys & 15)) * 8 * C::NX; i += 32) {
+                const int r = last_keys + i / (8 * C::NX), c = i % (8 * C::NX);
+                *reinterpret_cast<uint4*>(v + (c >> 3) * kKeys * 128 + r * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&B.vclean);
+        }
+      }
+    } else if (tile >= 0) {  // (the grid is sized without reading the bounds, and holds more blocks than query tiles)
         // ---------------- softmax: a thread a row ----------------
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
         const int i = warp >> 2;
         const int r = (warp & 3) * 32 + lane;
         const int lt = r / A.pack, lh = r % A.pack;
@@ -434,83 +522,82 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefill_kernel(const __grid_
         float m = -INFINITY, l = 0.f;
         bool ok = true;
         for (int j = 0; j < tiles; ++j) {
-            ok = mbar_wait_bounded(&B.sfull[i], j & 1, abort);
+            ok = wait_bar(&B.sfull[i], j & 1, abort);
             if (!__all_sync(0xffffffffu, ok)) {
                 gave_up();
                 ok = false;
                 break;
             }
             fence_after();
-            // S is read twice, 32 columns at a time (maximum, then weights): held whole, it would
-            // take 128 registers
-            const bool diagonal = j * kKeys + kKeys - 1 > lim0;
-            const int cut = lim - j * kKeys;  // columns past it are not seen
-            auto hide = [&](uint32_t* s, int x0) {
+            uint32_t sv[kKeys];
 #pragma unroll
-                for (int x = 0; x < 32; ++x)
-                    if (x0 + x > cut) s[x] = 0xff800000u;
-            };
-            float mx[4] = {m, m, m, m};
-            {
-                uint32_t s[2][32];
-                ld32(s[0], sa);
+            for (int x = 0; x < 4; ++x) ld32(sv + x * 32, sa + x * 32);
+            wait_ld();
+            if (j * kKeys + kKeys - 1 > lim0) {
+                const int cut = lim - j * kKeys;  // columns past it are not seen
 #pragma unroll
-                for (int x = 0; x < 4; ++x) {
-                    wait_ld();
-                    if (x < 3) ld32(s[(x + 1) & 1], sa + (x + 1) * 32);
-                    if (diagonal) hide(s[x & 1], x * 32);
-#pragma unroll
-                    for (int y = 0; y < 32; ++y) mx[y & 3] = fmaxf(mx[y & 3], __uint_as_float(s[x & 1][y]));
-                }
+                for (int x = 0; x < kKeys; ++x)
+                    if (x > cut) sv[x] = 0xff800000u;
             }
-            const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+            float mx[4] = {m, m, m, m};
+#pragma unroll
+            for (int x = 0; x < kKeys; x += 8)
+#pragma unroll
+                for (int y = 0; y < 4; ++y)
+                    mx[y] = max3(mx[y], __uint_as_float(sv[x + 2 * y]), __uint_as_float(sv[x + 2 * y + 1]));
+            const float top = max3(mx[0], mx[1], max3(mx[2], mx[2], mx[3]));
             if (j == 0) {
                 m = top;
-            } else if (__any_sync(0xffffffffu, (top - m) * c > kSlack)) {
+            } else if (__any_sync(0xffffffffu, live && !((top - m) * c <= kSlack))) {
                 // the products into O behind this tile's S have finished: S's completion covers them
                 const float a = top == m ? 1.f : ex2((m - top) * c);
                 m = top;
                 l *= a;
-#pragma unroll
-                for (int x = 0; x < D / 32; ++x) {
-                    uint32_t o[32];
-                    ld32(o, oa + x * 32);
+#pragma unroll 1
+                for (int x = 0; x < D / 16; ++x) {
+                    uint32_t o[16];
+                    ld16(o, oa + x * 16);
                     wait_ld();
 #pragma unroll
-                    for (int y = 0; y < 32; ++y) o[y] = __float_as_uint(__uint_as_float(o[y]) * a);
-                    st32(oa + x * 32, o);
+                    for (int y = 0; y < 16; ++y) o[y] = __float_as_uint(__uint_as_float(o[y]) * a);
+                    st16(oa + x * 16, o);
                 }
             }
             const float mc = m == -INFINITY ? 0.f : m * c;
-            float sum[2] = {0.f, 0.f};
-            {
-                uint32_t s[2][32];
-                ld32(s[0], sa);
+            const f2 cc = pair(c, c), mm = pair(-mc, -mc);
+            f2 sum0 = 0, sum1 = 0;
 #pragma unroll
-                for (int x = 0; x < 4; ++x) {
-                    wait_ld();
-                    if (x < 3) ld32(s[(x + 1) & 1], sa + (x + 1) * 32);
-                    if (diagonal) hide(s[x & 1], x * 32);
-                    uint32_t pk[16];
+            for (int x = 0; x < 4; ++x) {
+                uint32_t pk[16];
 #pragma unroll
-                    for (int y = 0; y < 16; ++y) {
-                        const float e0 = ex2(__fmaf_rn(__uint_as_float(s[x & 1][2 * y]), c, -mc));
-                        const float e1 = ex2(__fmaf_rn(__uint_as_float(s[x & 1][2 * y + 1]), c, -mc));
-                        sum[0] += e0;
-                        sum[1] += e1;
-                        pk[y] = pack_bf16(e0, e1);  // the second product's operand; its sums stay in f32
+                for (int y = 0; y < 16; ++y) {
+                    const f2 t = fma2(pair(__uint_as_float(sv[x * 32 + 2 * y]), __uint_as_float(sv[x * 32 + 2 * y + 1])), cc, mm);
+                    float e0, e1;
+                    if (y % kPolyOf == kPolyOf - 1) {
+                        exp2_pair(t, e0, e1);
+                    } else {
+                        unpair(t, e0, e1);
+                        e0 = ex2(e0);
+                        e1 = ex2(e1);
                     }
-                    st16(sa + x * 16, pk);  // over columns that have been read
+                    if (y & 1) sum1 = add2(sum1, pair(e0, e1));
+                    else sum0 = add2(sum0, pair(e0, e1));
+                    pk[y] = pack_bf16(e0, e1);  // the second product's operand; its sums stay in f32
+                }
+                st16(sa + x * 16, pk);  // over columns that are in registers by now
+                if (x & 1) {
+                    wait_st();
+                    fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&B.pready[i][x >> 1]);
                 }
             }
-            l += sum[0] + sum[1];
-            wait_st();
-            fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&B.pready[i]);
+            float e0, e1;
+            unpair(add2(sum0, sum1), e0, e1);
+            l += e0 + e1;
         }
         if (ok && tiles > 0) {
-            ok = mbar_wait_bounded(&B.odone[i], 0, abort);
+            ok = wait_bar(&B.odone[i], 0, abort);
             if (!__all_sync(0xffffffffu, ok)) {
                 gave_up();
                 ok = false;
@@ -518,7 +605,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefill_kernel(const __grid_
             fence_after();
         }
         if (ok) {
-            const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
+            // no key seen (m of a row without one is -inf, and exp2_pair's floor is not 0): zeros
+            const float inv = m == -INFINITY ? 0.f : 1.f / l;
             uint4* dst = reinterpret_cast<uint4*>(
                 p.out + ((uint64_t)(q0 + t) * p.q_heads + (uint64_t)kh * A.group + head0 + lh) * D);
 #pragma unroll
