@@ -91,6 +91,9 @@ __host__ __device__ constexpr uint32_t idesc(int M, int N, bool bmn) {
     return (1u << 4) | (1u << 7) | (1u << 10) | (bmn ? 1u << 16 : 0u) | ((uint32_t)(N >> 3) << 17) |
            ((uint32_t)(M >> 4) << 24);
 }
+// A value that is the same in every lane, as one the compiler knows to be.
+__device__ __forceinline__ int uniform(int x) { return __shfl_sync(0xffffffffu, x, 0); }
+
 // The issuing warp runs converged and one elected lane issues: with warp-uniform operands the
 // descriptors stay in uniform registers (issued from a divergent branch, a product cost some 100 cycles
 // more than it took the tensor pipe).
@@ -304,7 +307,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefill_kernel(const __grid_
     uint8_t* sq = raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u);
     uint8_t* skv = sq + 2 * C::QBYTES;
     __shared__ Bars B;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
     const int heads = (int)p.kv_heads * A.htiles;
     const int hi = (int)(blockIdx.x % heads), rank = (int)(blockIdx.x / heads);
     const int kh = hi / A.htiles, head0 = (hi % A.htiles) * A.pack;  // first query head of the group's pass
@@ -340,9 +343,9 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefill_kernel(const __grid_
     fence_before();
     __syncthreads();
     fence_after();
-    const uint32_t tmem = B.tmem;
+    const uint32_t tmem = (uint32_t)uniform((int)B.tmem);
     volatile int* abort = &B.abort;
-    const int tile = B.tile, nq = B.nq, nk = B.nk, q0 = B.q0, k0 = B.k0;
+    const int tile = uniform(B.tile), nq = uniform(B.nq), nk = uniform(B.nk), q0 = uniform(B.q0), k0 = uniform(B.k0);
 
     // key tiles of each query tile: up to its last token's limit
     int n[2], tok[2];
@@ -406,7 +409,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefill_kernel(const __grid_
       } else if (tile >= 0 && warp == 9) {
         // ---------------- MMA ----------------
         constexpr uint32_t IDS = idesc(128, kKeys, false), IDO = idesc(128, D, true);
-        const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+        const uint32_t tm = tmem;
         const uint64_t dq = desc_k(smem_u32(sq)), dk = desc_k(smem_u32(skv));
         const uint64_t dv = desc_mn(smem_u32(skv), kKeys * 128);
         auto wait = [&](uint64_t* bar, uint32_t parity) {
