@@ -138,6 +138,8 @@ def load(path: str = LIB_PATH) -> ctypes.CDLL:
     """Load the library and declare every exported signature.  Raises if the
     library or any declared symbol is missing."""
     global _lib
+    if _lib is not None:
+        return _lib
     with _lock:
         if _lib is not None:
             return _lib

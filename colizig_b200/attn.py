@@ -28,18 +28,27 @@ HEAD_DIMS = (64, 128)
 E4M3 = torch.float8_e4m3fn
 
 
+# A decode step is a few microseconds on the device: the checks below read each attribute
+# once and build messages only when something is wrong.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+_F32, _BF16, _I32, _I64 = torch.float32, torch.bfloat16, torch.int32, torch.int64
+
+
 def _ready() -> None:
     if not gpu.available():
         gpu.init()
 
 
-def _stream(stream, tensors) -> int:
+def _current(index: int) -> int:
+    """Handle of torch's current stream on device `index`."""
+    return _raw_stream(index) if _raw_stream is not None else torch.cuda.current_stream(index).cuda_stream
+
+
+def _stream(stream, index: int, tensors) -> int:
     """The stream's handle; tensors used on another stream than the current one are marked."""
-    if stream is None:
-        return torch.cuda.current_stream().cuda_stream
     handle = getattr(stream, "cuda_stream", stream)
-    if handle != torch.cuda.current_stream().cuda_stream:
-        s = stream if isinstance(stream, torch.cuda.Stream) else torch.cuda.ExternalStream(handle)
+    if handle != _current(index):
+        s = stream if isinstance(stream, torch.cuda.Stream) else torch.cuda.ExternalStream(handle, device=index)
         for t in tensors:
             if t is not None:
                 t.record_stream(s)
@@ -51,48 +60,60 @@ def _need(ok: bool, what: str) -> None:
         raise ValueError(what)
 
 
-def _rows(name: str, t: torch.Tensor, heads: Optional[int], dim: int, dtypes, device) -> int:
-    """Checks [rows, heads, dim] with packed heads and any 16-byte aligned row stride;
-    returns the row stride in elements."""
-    shape, st = t.shape, t.stride()
-    if not (len(shape) == 3 and shape[2] == dim and (heads is None or shape[1] == heads)):
-        raise ValueError(f"{name} must be [rows, {heads if heads is not None else 'heads'}, {dim}], got {tuple(shape)}")
-    if t.dtype not in dtypes:
-        raise ValueError(f"{name} must be one of {dtypes}, got {t.dtype}")
-    if t.device != device:
-        raise ValueError(f"{name} must be on {device}, got {t.device}")
-    row = shape[1] * dim
-    if st[2] != 1 or (shape[1] > 1 and st[1] != dim):
-        raise ValueError(f"{name}: heads of a row must be packed")
-    stride = st[0] if shape[0] > 1 else row  # one row (or none): its stride is never used
-    if stride < row or (stride * t.element_size()) & 15 or t.data_ptr() & 15:
-        raise ValueError(f"{name}: rows must be 16-byte aligned and must not overlap")
-    return stride
+def _rows(name: str, t: torch.Tensor, heads: Optional[int], dim: int, dtype, index: int):
+    """Checks [rows, heads, dim] with packed heads and any 16-byte aligned row stride; returns
+    (rows, heads, row stride in elements, address)."""
+    shape = t.shape
+    if len(shape) == 3 and t.dtype is dtype and t.get_device() == index:
+        n, h, d = shape
+        s0, s1, s2 = t.stride()
+        if d == dim and (h == heads or heads is None) and s2 == 1 and (s1 == dim or h <= 1):
+            at = t.data_ptr()
+            if n <= 1:
+                s0 = h * dim  # one row (or none): its stride is never used
+            if s0 >= h * dim and not (s0 * (4 if dtype is _F32 else 2) | at) & 15:
+                return n, h, s0, at
+            raise ValueError(f"{name}: rows must be 16-byte aligned and must not overlap")
+    raise ValueError(f"{name} must be {dtype} [rows, {heads if heads is not None else 'heads'}, {dim}] with packed heads "
+                     f"on cuda:{index}, got {t.dtype} {tuple(shape)} (strides {t.stride()}) on {t.device}")
 
 
-def _ints(name: str, t: torch.Tensor, shape, dtype, device) -> int:
-    if t.dtype != dtype or t.shape != shape or t.device != device or not t.is_contiguous():
-        raise ValueError(f"{name} must be a contiguous {dtype} tensor {tuple(shape)} on {device}, "
-                         f"got {t.dtype} {tuple(t.shape)} on {t.device}")
-    return t.data_ptr()
+def _ints(name: str, t: torch.Tensor, n: int, dtype, index: int) -> int:
+    shape = t.shape
+    if len(shape) == 1 and shape[0] == n and t.dtype is dtype and t.get_device() == index and \
+            (n <= 1 or t.stride(0) == 1):
+        return t.data_ptr()
+    raise ValueError(f"{name} must be a packed {dtype} tensor [{n}] on cuda:{index}, got {t.dtype} {tuple(shape)} on "
+                     f"{t.device}")
 
 
-def _vector(name: str, t: Optional[torch.Tensor], n: int, device) -> Optional[int]:
+def _vector(name: str, t: Optional[torch.Tensor], n: int, index: int) -> Optional[int]:
     if t is None:
         return None
-    if t.dtype != torch.float32 or tuple(t.shape) != (n,) or t.device != device or t.stride(0) != 1 or \
-            t.data_ptr() & 15:
-        raise ValueError(f"{name} must be a packed, 16-byte aligned f32 [{n}] tensor on {device}")
-    return t.data_ptr()
+    shape = t.shape
+    if len(shape) == 1 and shape[0] == n and t.dtype is _F32 and t.get_device() == index and t.stride(0) == 1:
+        at = t.data_ptr()
+        if not at & 15:
+            return at
+    raise ValueError(f"{name} must be a packed, 16-byte aligned f32 [{n}] tensor on cuda:{index}, got {t.dtype} "
+                     f"{tuple(shape)} on {t.device}")
 
 
-def _output(name: str, t: Optional[torch.Tensor], shape, like: torch.Tensor) -> torch.Tensor:
+def _output(name: str, t: Optional[torch.Tensor], n: int, heads: int, dim: int, like: torch.Tensor, index: int):
+    """(t, its address), or a new tensor like `like` in bf16 when t is None."""
     if t is None:
-        return torch.empty(shape, dtype=torch.bfloat16, device=like.device)
-    if t.dtype != torch.bfloat16 or tuple(t.shape) != tuple(shape) or t.device != like.device or \
-            not t.is_contiguous() or t.data_ptr() & 15:
-        raise ValueError(f"{name} must be a contiguous, 16-byte aligned bf16 tensor {tuple(shape)} on {like.device}")
-    return t
+        if like.dtype is not _BF16:
+            t = torch.empty((n, heads, dim), dtype=_BF16, device=like.device)
+        elif like.is_contiguous():
+            t = torch.empty_like(like)
+        else:
+            t = like.new_empty((n, heads, dim))
+        return t, t.data_ptr()
+    if t.dtype is not _BF16 or t.shape != (n, heads, dim) or t.get_device() != index or not t.is_contiguous() or \
+            t.data_ptr() & 15:
+        raise ValueError(f"{name} must be a contiguous, 16-byte aligned bf16 tensor {(n, heads, dim)} on cuda:{index}, "
+                         f"got {t.dtype} {tuple(t.shape)} on {t.device}")
+    return t, t.data_ptr()
 
 
 class KvCache:
@@ -126,7 +147,7 @@ class KvCache:
                                 t.is_contiguous()), f"{name} must be a contiguous f32 [{hk}] tensor on {k.device}")
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
         self.pages, self.kv_heads, self.page_size, self.head_dim = pages, hk, page, d
-        self.device = k.device
+        self.device, self._index = k.device, k.get_device()
         self._c = _abi.KvCacheC(k.data_ptr(), v.data_ptr(), None if k_scale is None else k_scale.data_ptr(),
                                 None if v_scale is None else v_scale.data_ptr(), strides[0], strides[1], pages, page,
                                 hk, d, _abi.COLIZIG_KV_E4M3 if e4m3 else _abi.COLIZIG_KV_BF16)
@@ -157,42 +178,38 @@ def append(cache: KvCache, q, k, v, positions, slots, rope=None, q_norm=None, k_
     slices of a fused projection as they are); k and v go to cache row slots[t] (i64; page *
     page_size + row, negative: not cached, no slot twice), positions i32 [T].  Returns (q, k, v)
     packed in bf16; k and v (what ``prefill`` reads) are None unless packed or given."""
-    dev, d, hk = cache.device, cache.head_dim, cache.kv_heads
-    dts = (q.dtype,) if q.dtype in (torch.float32, torch.bfloat16) else (torch.float32, torch.bfloat16)
-    qs = _rows("q", q, None, d, dts, dev)
-    T, hq = q.shape[0], q.shape[1]
+    dev, d, hk = cache._index, cache.head_dim, cache.kv_heads
+    dt = _F32 if q.dtype is _F32 else _BF16
+    T, hq, qs, qp = _rows("q", q, None, d, dt, dev)
     if hq < 1 or hq % hk:
         raise ValueError(f"{hq} query heads are not a multiple of {hk} key/value heads")
-    ks = _rows("k", k, hk, d, dts, dev)
-    vs = _rows("v", v, hk, d, dts, dev)
-    if k.shape[0] != T or v.shape[0] != T:
+    tk, _, ks, kp = _rows("k", k, hk, d, dt, dev)
+    tv, _, vs, vp = _rows("v", v, hk, d, dt, dev)
+    if tk != T or tv != T:
         raise ValueError("q, k and v must hold the same tokens")
-    sp = _ints("slots", slots, (T,), torch.int64, dev)
+    sp = _ints("slots", slots, T, _I64, dev)
     rp, rlen, rot, pp = None, 0, 0, None
     if rope is not None:
-        rlen, rot = rope.shape
-        if rope.dtype != torch.float32 or rope.device != dev or not rope.is_contiguous() or rope.data_ptr() & 15 or \
-                rot % 16 or not 0 < rot <= d or rlen < 1:
-            raise ValueError(f"rope must be a contiguous f32 [positions, rot_dim] table on {dev}, rot_dim a multiple "
-                             f"of 16 up to {d}")
-        pp = _ints("positions", positions, (T,), torch.int32, dev)
+        shape = rope.shape
+        if len(shape) != 2 or rope.dtype is not _F32 or rope.get_device() != dev or not rope.is_contiguous() or \
+                rope.data_ptr() & 15 or shape[1] % 16 or not 0 < shape[1] <= d or shape[0] < 1:
+            raise ValueError(f"rope must be a contiguous f32 [positions, rot_dim] table on cuda:{dev}, rot_dim a "
+                             f"multiple of 16 up to {d}")
+        rlen, rot = shape
         rp = rope.data_ptr()
+        pp = _ints("positions", positions, T, _I32, dev)
     qn, kn = _vector("q_norm", q_norm, d, dev), _vector("k_norm", k_norm, d, dev)
-    handle = _stream(stream, (q, k, v, positions, slots, rope, q_norm, k_norm, cache.k, cache.v, cache.k_scale,
-                              cache.v_scale, q_out, k_out, v_out)) if stream is not None else \
-        torch.cuda.current_stream().cuda_stream
-    q_out = _output("q_out", q_out, (T, hq, d), q)
+    kop = vop = None
+    q_out, qop = _output("q_out", q_out, T, hq, d, q, dev)
     if packed or k_out is not None:
-        k_out = _output("k_out", k_out, (T, hk, d), q)
+        k_out, kop = _output("k_out", k_out, T, hk, d, k, dev)
     if packed or v_out is not None:
-        v_out = _output("v_out", v_out, (T, hk, d), q)
-    if stream is not None:
-        _stream(stream, (q_out, k_out, v_out))
-    rc = _abi.load().colizig_cuda_attn_append(
-        cache._ref, q.data_ptr(), k.data_ptr(), v.data_ptr(),
-        _abi.COLIZIG_X_BF16 if q.dtype == torch.bfloat16 else _abi.COLIZIG_X_F32, T, hq, qs, ks, vs, pp, sp, rp, rlen,
-        rot, qn, kn, eps, q_out.data_ptr(), None if k_out is None else k_out.data_ptr(),
-        None if v_out is None else v_out.data_ptr(), handle)
+        v_out, vop = _output("v_out", v_out, T, hk, d, v, dev)
+    handle = _current(dev) if stream is None else _stream(stream, dev, (
+        q, k, v, positions, slots, rope, q_norm, k_norm, cache.k, cache.v, cache.k_scale, cache.v_scale, q_out, k_out,
+        v_out))
+    rc = _abi.load().colizig_cuda_attn_append(cache._ref, qp, kp, vp, 0 if dt is _F32 else 1, T, hq, qs, ks, vs, pp, sp,
+                                              rp, rlen, rot, qn, kn, eps, qop, kop, vop, handle)
     if rc:
         _abi.check("colizig_cuda_attn_append", rc)
     return q_out, k_out, v_out
@@ -214,30 +231,31 @@ class DecodePlan:
         self._fn = L.colizig_cuda_attn_decode
         with torch.cuda.device(cache.device):
             self._ws = torch.zeros(L.colizig_cuda_attn_decode_workspace(), dtype=torch.uint8, device=cache.device)
+        self._wsp = self._ws.data_ptr()
 
     def run(self, q, table, lens, out=None, stream=None):
         """out [B, q_heads, head_dim] bf16 = attention of q (bf16, row stride free) over the lens[b]
         first tokens of the pages table[b] (i32 [B, width], row stride free; lens i32 [B])."""
         c = self.cache
-        qs = _rows("q", q, self.q_heads, c.head_dim, (torch.bfloat16,), c.device)
-        B = q.shape[0]
+        dev, d, hq = c._index, c.head_dim, self.q_heads
+        B, _, qs, qp = _rows("q", q, hq, d, _BF16, dev)
         if B > self.max_batch:
             raise ValueError(f"{B} sequences, the plan holds {self.max_batch}")
-        if table.dtype != torch.int32 or table.dim() != 2 or table.shape[0] != B or table.device != c.device or \
-                table.shape[1] < 1 or table.stride(1) != 1 or (B > 1 and table.stride(0) < table.shape[1]):
-            raise ValueError(f"table must be an i32 tensor [{B}, width] on {c.device}, got {table.dtype} "
-                             f"{tuple(table.shape)}")
-        lp = _ints("lens", lens, (B,), torch.int32, c.device)
-        if stream is None:
-            handle = torch.cuda.current_stream().cuda_stream
-        else:
-            handle = _stream(stream, (q, table, lens, out, c.k, c.v, c.k_scale, c.v_scale, self._ws))
-        out = _output("out", out, (B, self.q_heads, c.head_dim), q)
-        if stream is not None:
-            _stream(stream, (out,))
-        rc = self._fn(c._ref, q.data_ptr(), qs, B, self.q_heads, table.data_ptr(), table.shape[1],
-                      table.stride(0) if B > 1 else table.shape[1], lp, self.scale, out.data_ptr(),
-                      self._ws.data_ptr(), handle)
+        shape = table.shape
+        if len(shape) != 2 or shape[0] != B or shape[1] < 1 or table.dtype is not _I32 or table.get_device() != dev:
+            raise ValueError(f"table must be an i32 tensor [{B}, width] on cuda:{dev}, got {table.dtype} {tuple(shape)} "
+                             f"on {table.device}")
+        width = shape[1]
+        t0, t1 = table.stride()
+        if B <= 1:
+            t0 = width
+        if (t1 != 1 and width > 1) or t0 < width:
+            raise ValueError(f"table: rows must be packed and must not overlap, strides {table.stride()}")
+        lp = _ints("lens", lens, B, _I32, dev)
+        out, op = _output("out", out, B, hq, d, q, dev)
+        handle = _current(dev) if stream is None else _stream(stream, dev, (
+            q, table, lens, out, c.k, c.v, c.k_scale, c.v_scale, self._ws))
+        rc = self._fn(c._ref, qp, qs, B, hq, table.data_ptr(), width, t0, lp, self.scale, op, self._wsp, handle)
         if rc:
             _abi.check("colizig_cuda_attn_decode", rc)
         return out
@@ -249,32 +267,26 @@ def prefill(q, k, v, cu_q, cu_k=None, scale: Optional[float] = None, out=None, s
     strides free; cu i32 [B + 1], cu_k defaults to cu_q).  Queries are the last tokens of
     their sequence; a query that sees no key gives zeros.  scale defaults to head_dim ** -0.5."""
     _ready()
-    dev = q.device
-    d = q.shape[-1]
-    if not q.is_cuda or d not in HEAD_DIMS:
-        raise ValueError(f"q must be a CUDA tensor of head_dim {HEAD_DIMS}, got {tuple(q.shape)} on {dev}")
-    bf = (torch.bfloat16,)
-    qs = _rows("q", q, None, d, bf, dev)
-    ks = _rows("k", k, None, d, bf, dev)
-    hq, hk = q.shape[1], k.shape[1]
-    vs = _rows("v", v, hk, d, bf, dev)
-    if hk < 1 or hq < 1 or hq % hk or v.shape[0] != k.shape[0]:
+    dev, d = q.get_device(), q.shape[-1]
+    if dev < 0 or d not in HEAD_DIMS:
+        raise ValueError(f"q must be a CUDA tensor of head_dim {HEAD_DIMS}, got {tuple(q.shape)} on {q.device}")
+    Tq, hq, qs, qp = _rows("q", q, None, d, _BF16, dev)
+    Tk, hk, ks, kp = _rows("k", k, None, d, _BF16, dev)
+    tv, _, vs, vp = _rows("v", v, hk, d, _BF16, dev)
+    if hk < 1 or hq < 1 or hq % hk or tv != Tk:
         raise ValueError(f"q {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)} do not belong together")
     if cu_k is None:
         cu_k = cu_q
-        if k.shape[0] != q.shape[0]:
+        if Tk != Tq:
             raise ValueError("without cu_k, q and k must hold the same tokens")
     n = cu_q.shape[0]
     if n < 1:
         raise ValueError("cu_q must hold at least the leading 0")
-    cq, ck = _ints("cu_q", cu_q, (n,), torch.int32, dev), _ints("cu_k", cu_k, (n,), torch.int32, dev)
-    handle = torch.cuda.current_stream().cuda_stream if stream is None else _stream(stream, (q, k, v, cu_q, cu_k, out))
-    out = _output("out", out, (q.shape[0], hq, d), q)
-    if stream is not None:
-        _stream(stream, (out,))
-    rc = _abi.load().colizig_cuda_attn_prefill(q.data_ptr(), k.data_ptr(), v.data_ptr(), qs, ks, vs, q.shape[0],
-                                               k.shape[0], n - 1, hq, hk, d, cq, ck,
-                                               d ** -0.5 if scale is None else scale, out.data_ptr(), handle)
+    cq, ck = _ints("cu_q", cu_q, n, _I32, dev), _ints("cu_k", cu_k, n, _I32, dev)
+    out, op = _output("out", out, Tq, hq, d, q, dev)
+    handle = _current(dev) if stream is None else _stream(stream, dev, (q, k, v, cu_q, cu_k, out))
+    rc = _abi.load().colizig_cuda_attn_prefill(qp, kp, vp, qs, ks, vs, Tq, Tk, n - 1, hq, hk, d, cq, ck,
+                                               d ** -0.5 if scale is None else scale, op, handle)
     if rc:
         _abi.check("colizig_cuda_attn_prefill", rc)
     return out
@@ -283,5 +295,5 @@ def prefill(q, k, v, cu_q, cu_k=None, scale: Optional[float] = None, out=None, s
 def check(stream=None) -> None:
     """Raise if an attention call since the last check met an index outside its buffer (slot,
     position, page, length or sequence bound).  Waits for `stream` (default: the current one)."""
-    handle = torch.cuda.current_stream().cuda_stream if stream is None else getattr(stream, "cuda_stream", stream)
+    handle = _current(torch.cuda.current_device()) if stream is None else getattr(stream, "cuda_stream", stream)
     _abi.check("colizig_cuda_attn_check", _abi.load().colizig_cuda_attn_check(handle))

@@ -33,10 +33,6 @@ constexpr uint32_t kTmemCols = 512;
 // above it: P and l then grow to at most 2^8, far inside f32 and bf16, and most tiles
 // rescale nothing.  The result does not depend on it (o and l share the factor).
 constexpr float kSlack = 8.f;
-// Of every kPolyOf pairs of weights one is computed on the FMA pipe (exp2_pair), the rest by ex2: the
-// exponentials of two tiles would keep the special-function pipe as busy as the products keep the
-// tensor pipe.
-constexpr int kPolyOf = 4;
 
 struct PrefillArgs {
     CUtensorMap qmap, kmap, vmap;  // [rows][heads][D] in boxes of 64 columns
@@ -171,23 +167,6 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     float r;
     asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
     return r;
-}
-// 2^t of two t <= 16 without the special-function pipe: t = n + f, n whole, |f| <= 1/2; 2^f by
-// the cubic of least largest relative error on that interval (Remez exchange, 7.5e-5, a
-// fiftieth of the rounding to bf16 that follows), n into the exponent.  t under -126 counts as -126.
-__device__ __forceinline__ void exp2_pair(f2 t, float& a, float& b) {
-    unpair(t, a, b);
-    const f2 x = pair(fmaxf(a, -126.f), fmaxf(b, -126.f));
-    const f2 u = add2(x, pair(12582912.f, 12582912.f));  // 1.5 * 2^23: n in the low bits
-    const f2 f = add2(x, fma2(u, pair(-1.f, -1.f), pair(12582912.f, 12582912.f)));
-    f2 y = fma2(pair(0.0551716685295105f, 0.0551716685295105f), f, pair(0.2426111251115799f, 0.2426111251115799f));
-    y = fma2(y, f, pair(0.6932609677314758f, 0.6932609677314758f));
-    y = fma2(y, f, pair(0.9999280571937561f, 0.9999280571937561f));
-    float ua, ub;
-    unpair(u, ua, ub);
-    unpair(y, a, b);
-    a = __uint_as_float(__float_as_uint(a) + (__float_as_uint(ua) << 23));
-    b = __uint_as_float(__float_as_uint(b) + (__float_as_uint(ub) << 23));
 }
 // A bounded wait without calls (setmaxnreg and calls do not go together).
 __device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, const volatile int* abort) {
@@ -576,13 +555,9 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefill_kernel(const __grid_
                 for (int y = 0; y < 16; ++y) {
                     const f2 t = fma2(pair(__uint_as_float(sv[x * 32 + 2 * y]), __uint_as_float(sv[x * 32 + 2 * y + 1])), cc, mm);
                     float e0, e1;
-                    if (y % kPolyOf == kPolyOf - 1) {
-                        exp2_pair(t, e0, e1);
-                    } else {
-                        unpair(t, e0, e1);
-                        e0 = ex2(e0);
-                        e1 = ex2(e1);
-                    }
+                    unpair(t, e0, e1);
+                    e0 = ex2(e0);
+                    e1 = ex2(e1);
                     if (y & 1) sum1 = add2(sum1, pair(e0, e1));
                     else sum0 = add2(sum0, pair(e0, e1));
                     pk[y] = pack_bf16(e0, e1);  // the second product's operand; its sums stay in f32
@@ -608,8 +583,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefill_kernel(const __grid_
             fence_after();
         }
         if (ok) {
-            // no key seen (m of a row without one is -inf, and exp2_pair's floor is not 0): zeros
-            const float inv = m == -INFINITY ? 0.f : 1.f / l;
+            const float inv = m == -INFINITY ? 0.f : 1.f / l;  // no key seen: zeros
             uint4* dst = reinterpret_cast<uint4*>(
                 p.out + ((uint64_t)(q0 + t) * p.q_heads + (uint64_t)kh * A.group + head0 + lh) * D);
 #pragma unroll
