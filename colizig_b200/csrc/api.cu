@@ -1801,7 +1801,7 @@ int kv_view(const colizig_kv_cache* c, cz::KvView& v) {
     const uint64_t elt = c->dtype == COLIZIG_KV_BF16 ? 2 : 1;
     if (elt == 2 && (c->k_scale || c->v_scale)) return CZ_EARGS;
     if (c->pages < 1 || c->kv_heads < 1 || c->page_size < 16 || c->page_size % 16 || c->page_size > 65536 ||
-        c->pages > 0x7fffffffu || c->kv_heads > 65535 || (c->head_dim != 64 && c->head_dim != 128))
+        (uint64_t)c->pages * c->page_size > 0xffffffffu || c->pages > 0x7fffffffu || c->kv_heads > 65535 || (c->head_dim != 64 && c->head_dim != 128))
         return CZ_ESHAPE;
     const uint64_t page = (uint64_t)c->kv_heads * c->page_size * c->head_dim;
     if (c->k_page_stride < page || c->v_page_stride < page || c->k_page_stride * elt % 16 ||
@@ -1871,7 +1871,7 @@ CZ_EXPORT int colizig_cuda_attn_append(const colizig_kv_cache* cache, const void
     p.v_out = reinterpret_cast<uint16_t*>(v_out);
     p.err = g.attn_err;
     cudaSetDevice(g.dev);
-    return cz::attn_append_launch(p, reinterpret_cast<cudaStream_t>(stream));
+    return cz::attn_append_launch(p, g.num_sms, reinterpret_cast<cudaStream_t>(stream));
 }
 
 CZ_EXPORT size_t colizig_cuda_attn_decode_workspace(void) {

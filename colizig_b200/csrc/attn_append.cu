@@ -8,11 +8,17 @@
 // All arithmetic is f32; one rounding at the store (bf16, or E4M3 of x / scale,
 // saturated), which is the cache's own type.
 //
-// D / 8 lanes share a head, 8 elements each (two 16-byte loads of f32 or one of
-// bf16, one 16-byte store); the sum of squares and the rotation partner, R/2
-// elements away = R/16 lanes, go through shuffles, so nothing is staged.  A
-// group of lanes takes kHeads heads of one token, whose loads are all in
-// flight together and share the token's cosines and sines in registers.
+// D / 8 lanes share a head.  A lane holds four consecutive elements and the four they are
+// turned with (R/2 further on; beyond the rotated part, two runs of four that are left as they
+// are), so that the rotation needs no exchange and a lane reads four cosines and four sines;
+// only the sum of squares goes through shuffles.  A group of lanes takes four heads of one
+// token (two when that would leave SMs without a block), whose loads are all in flight together
+// and share the cosines and sines.
+//
+// Bound by memory: 8,192 tokens of 32 + 2 x 4 heads of 128 in f32 to bf16, with packed copies, are 272 MB
+// and take 56 us, 4.86 TB/s (0.75 of a copy's rate).  Four heads against two: 56.0 and 56.1 us there,
+// 5.9 and 6.7 us for 1,531 tokens of 16 + 32 heads of 64 in bf16; for 96 tokens 4.2 and 3.5 us, for one 3.7
+// and 3.0 us.
 #include <cuda_bf16.h>
 #include <cuda_fp8.h>
 #include <cuda_runtime.h>
@@ -24,173 +30,170 @@
 namespace cz {
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 128;
 
+// Four elements, read once: not kept in L1 (the rotation table is).
 template <int XBF16>
-__device__ __forceinline__ void load8(const void* base, uint64_t at, float* f) {
+__device__ __forceinline__ void load4(const void* base, uint64_t at, float* f) {
     if (XBF16) {
-        const uint4 r = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(base) + at));
-        const uint32_t w[4] = {r.x, r.y, r.z, r.w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            f[2 * i] = __uint_as_float(w[i] << 16);
-            f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-        }
+        uint2 r;
+        asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0, %1}, [%2];"
+                     : "=r"(r.x), "=r"(r.y)
+                     : "l"(reinterpret_cast<const uint16_t*>(base) + at));
+        f[0] = __uint_as_float(r.x << 16), f[1] = __uint_as_float(r.x & 0xffff0000u);
+        f[2] = __uint_as_float(r.y << 16), f[3] = __uint_as_float(r.y & 0xffff0000u);
     } else {
-        const float4* s = reinterpret_cast<const float4*>(reinterpret_cast<const float*>(base) + at);
-        const float4 a = __ldg(s), b = __ldg(s + 1);
-        f[0] = a.x, f[1] = a.y, f[2] = a.z, f[3] = a.w;
-        f[4] = b.x, f[5] = b.y, f[6] = b.z, f[7] = b.w;
+        asm volatile("ld.global.nc.L1::no_allocate.v4.f32 {%0, %1, %2, %3}, [%4];"
+                     : "=f"(f[0]), "=f"(f[1]), "=f"(f[2]), "=f"(f[3])
+                     : "l"(reinterpret_cast<const float*>(base) + at));
     }
 }
 
-__device__ __forceinline__ uint4 pack_bf16x8(const float* f) {
-    uint32_t w[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const __nv_bfloat162 h = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
-        w[i] = *reinterpret_cast<const uint32_t*>(&h);
-    }
-    return make_uint4(w[0], w[1], w[2], w[3]);
+__device__ __forceinline__ float4 ldg4(const float* p) { return __ldg(reinterpret_cast<const float4*>(p)); }
+
+__device__ __forceinline__ uint2 pack_bf16x4(const float* f) {
+    const __nv_bfloat162 a = __floats2bfloat162_rn(f[0], f[1]), b = __floats2bfloat162_rn(f[2], f[3]);
+    return make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
 }
 
 // E4M3 of x / scale, saturated at +-448 (NaN stays NaN).
-__device__ __forceinline__ uint2 pack_e4m3x8(const float* f, float scale) {
-    uint32_t w[2];
+__device__ __forceinline__ uint32_t pack_e4m3x4(const float* f, float scale) {
+    uint32_t u = 0;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        uint32_t u = 0;
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            const float2 v = make_float2(__fdiv_rn(f[4 * i + 2 * j], scale), __fdiv_rn(f[4 * i + 2 * j + 1], scale));
-            u |= (uint32_t)__nv_cvt_float2_to_fp8x2(v, __NV_SATFINITE, __NV_E4M3) << (16 * j);
-        }
-        w[i] = u;
+    for (int j = 0; j < 2; ++j) {
+        const float2 v = make_float2(__fdiv_rn(f[2 * j], scale), __fdiv_rn(f[2 * j + 1], scale));
+        u |= (uint32_t)__nv_cvt_float2_to_fp8x2(v, __NV_SATFINITE, __NV_E4M3) << (16 * j);
     }
-    return make_uint2(w[0], w[1]);
+    return u;
 }
 
 // D: head size; XBF16: projections are bf16; HEADS: heads of one token per group of lanes.
 template <int D, int XBF16, int HEADS>
-__global__ void __launch_bounds__(kThreads) attn_append_kernel(const AppendParams p) {
+__global__ void __launch_bounds__(kThreads, HEADS == 4 ? 8 : 10) attn_append_kernel(const AppendParams p) {
     constexpr int L = D / 8;
     const int sub = threadIdx.x % L;
     const uint32_t hq = p.q_heads, hk = p.kv.kv_heads;
     const uint32_t per_token = (hq + 2 * hk + HEADS - 1) / HEADS;  // groups of lanes
-    const uint64_t item = (uint64_t)blockIdx.x * (kThreads / L) + threadIdx.x / L;
-    const bool live = item < (uint64_t)p.T * per_token;  // the whole group agrees; dead groups still join the shuffles
-    const uint32_t t = live ? (uint32_t)(item / per_token) : 0;
-    const uint32_t g = live ? (uint32_t)(item % per_token) : 0;
+    const uint32_t item = blockIdx.x * (kThreads / L) + threadIdx.x / L;
+    const bool live = item < (uint32_t)p.T * per_token;  // the whole group agrees; dead groups still join the shuffles
+    const uint32_t t = live ? item / per_token : 0;
+    const uint32_t g = live ? item % per_token : 0;
+    // this lane's two runs of four
+    const int rot = (int)p.rot, turning = rot / 8;  // lanes of the rotated part
+    const bool turned = sub < turning;
+    const int e0 = turned ? 4 * sub : rot + 4 * (sub - turning);
+    const int e1 = e0 + (turned ? rot : D - rot) / 2;
 
+    int pos = turned && live ? __ldg(p.positions + t) : 0;
+    const int64_t slot = live ? __ldg(p.slots + t) : -1;
     float f[HEADS][8];
 #pragma unroll
     for (int j = 0; j < HEADS; ++j) {
         const uint32_t h = g + j * per_token;
-        if (!live || h >= hq + 2 * hk) {
+        const bool some = live && h < hq + 2 * hk;
+        const void* x = h < hq ? p.q : h < hq + hk ? p.k : p.v;
+        const uint64_t at = h < hq        ? t * p.q_stride + (uint64_t)h * D
+                            : h < hq + hk ? t * p.k_stride + (uint64_t)(h - hq) * D
+                                          : t * p.v_stride + (uint64_t)(h - hq - hk) * D;
+        if (some) {
+            load4<XBF16>(x, at + e0, f[j]);
+            load4<XBF16>(x, at + e1, f[j] + 4);
+        } else {
 #pragma unroll
             for (int i = 0; i < 8; ++i) f[j][i] = 0.f;
-        } else if (h < hq) {
-            load8<XBF16>(p.q, t * p.q_stride + (uint64_t)h * D + sub * 8, f[j]);
-        } else if (h < hq + hk) {
-            load8<XBF16>(p.k, t * p.k_stride + (uint64_t)(h - hq) * D + sub * 8, f[j]);
-        } else {
-            load8<XBF16>(p.v, t * p.v_stride + (uint64_t)(h - hq - hk) * D + sub * 8, f[j]);
         }
     }
-    // this lane's cosines and sines: elements 8 sub .. 8 sub + 7 lie in one half of the
-    // rotated part (R/2 is a multiple of 8); outside it c = 1, s = 0
-    float c[8], s[8];
-    const int half = (int)p.rot / 2;
-    const int e0 = sub * 8;
-    const bool turned = p.rot != 0 && e0 < (int)p.rot;
-    const bool upper = turned && e0 >= half;
-    const int partner = !turned ? sub : upper ? sub - half / 8 : sub + half / 8;
+    float4 c = make_float4(1.f, 1.f, 1.f, 1.f), s = make_float4(0.f, 0.f, 0.f, 0.f);
     if (turned) {
-        int pos = live ? __ldg(p.positions + t) : 0;
         if (pos < 0 || (uint32_t)pos >= p.rope_len) {
             atomicOr(p.err, kAttnErrIndex);
             pos = 0;
         }
-        const float* row = p.rope + (uint64_t)pos * p.rot + (e0 - (upper ? half : 0));
-        load8<0>(row, 0, c);
-        load8<0>(row, half, s);
-        if (!upper) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) s[i] = -s[i];
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) c[i] = 1.f, s[i] = 0.f;
+        const float* row = p.rope + (uint64_t)pos * rot + e0;
+        c = ldg4(row);
+        s = ldg4(row + rot / 2);
     }
-    const int64_t slot = live ? __ldg(p.slots + t) : -1;
     const bool in_cache = slot >= 0 && slot < (int64_t)p.kv.pages * p.kv.page_size;
     if (slot >= 0 && !in_cache && sub == 0) atomicOr(p.err, kAttnErrIndex);
-    const uint64_t page = in_cache ? (uint64_t)slot / p.kv.page_size : 0;
-    const uint64_t row = in_cache ? (uint64_t)slot % p.kv.page_size : 0;
+    const uint32_t page = in_cache ? (uint32_t)slot / p.kv.page_size : 0;  // (a cache has fewer than 2^32 rows)
+    const uint32_t row = in_cache ? (uint32_t)slot - page * p.kv.page_size : 0;
 
 #pragma unroll
     for (int j = 0; j < HEADS; ++j) {
         const uint32_t h = g + j * per_token;
         const bool is_v = h >= hq + hk;
+        float* y = f[j];
         const float* w = h < hq ? p.q_norm : is_v ? nullptr : p.k_norm;
-        float y[8];
-        float ss = 0.f;
+        if (p.q_norm || p.k_norm) {  // (all lanes agree, for the shuffles)
+            float ss = 0.f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) ss = __fmaf_rn(f[j][i], f[j][i], ss);
+            for (int i = 0; i < 8; ++i) ss = __fmaf_rn(y[i], y[i], ss);
 #pragma unroll
-        for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-        float wv[8];
-        if (w) {
-            load8<0>(w, e0, wv);
-            const float r = 1.f / sqrtf(ss * (1.f / D) + p.eps);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) y[i] = f[j][i] * r * wv[i];
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) y[i] = f[j][i];
+            for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+            if (w) {
+                const float4 w0 = ldg4(w + e0), w1 = ldg4(w + e1);
+                const float r = 1.f / sqrtf(ss * (1.f / D) + p.eps);
+                y[0] *= r * w0.x, y[1] *= r * w0.y, y[2] *= r * w0.z, y[3] *= r * w0.w;
+                y[4] *= r * w1.x, y[5] *= r * w1.y, y[6] *= r * w1.z, y[7] *= r * w1.w;
+            }
         }
+        if (!is_v && turned) {
+            const float cc[4] = {c.x, c.y, c.z, c.w}, sn[4] = {s.x, s.y, s.z, s.w};
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float o = __shfl_sync(0xffffffffu, y[i], partner, L);
-            if (!is_v && turned) y[i] = __fmaf_rn(o, s[i], y[i] * c[i]);
+            for (int i = 0; i < 4; ++i) {
+                const float a = y[i], b = y[i + 4];
+                y[i] = __fmaf_rn(a, cc[i], -b * sn[i]);
+                y[i + 4] = __fmaf_rn(b, cc[i], a * sn[i]);
+            }
         }
         if (!live || h >= hq + 2 * hk) continue;
+        const uint2 lo = pack_bf16x4(y), hi = pack_bf16x4(y + 4);
         if (h < hq) {
-            *reinterpret_cast<uint4*>(p.q_out + ((uint64_t)t * hq + h) * D + e0) = pack_bf16x8(y);
+            uint16_t* dst = p.q_out + ((uint64_t)t * hq + h) * D;
+            *reinterpret_cast<uint2*>(dst + e0) = lo;
+            *reinterpret_cast<uint2*>(dst + e1) = hi;
             continue;
         }
         const uint32_t kh = is_v ? h - hq - hk : h - hq;
         uint16_t* packed = is_v ? p.v_out : p.k_out;
-        const uint4 b = pack_bf16x8(y);
-        if (packed) *reinterpret_cast<uint4*>(packed + ((uint64_t)t * hk + kh) * D + e0) = b;
+        if (packed) {
+            packed += ((uint64_t)t * hk + kh) * D;
+            *reinterpret_cast<uint2*>(packed + e0) = lo;
+            *reinterpret_cast<uint2*>(packed + e1) = hi;
+        }
         if (!in_cache) continue;
-        const uint64_t at = page * (is_v ? p.kv.v_page : p.kv.k_page) + ((uint64_t)kh * p.kv.page_size + row) * D + e0;
+        const uint64_t at = (uint64_t)page * (is_v ? p.kv.v_page : p.kv.k_page) + ((uint64_t)kh * p.kv.page_size + row) * D;
         uint8_t* base = is_v ? p.kv.v : p.kv.k;
         if (p.kv.e4m3) {
             const float* sc = is_v ? p.kv.v_scale : p.kv.k_scale;
-            *reinterpret_cast<uint2*>(base + at) = pack_e4m3x8(y, sc ? __ldg(sc + kh) : 1.f);
+            const float scale = sc ? __ldg(sc + kh) : 1.f;
+            *reinterpret_cast<uint32_t*>(base + at + e0) = pack_e4m3x4(y, scale);
+            *reinterpret_cast<uint32_t*>(base + at + e1) = pack_e4m3x4(y + 4, scale);
         } else {
-            *reinterpret_cast<uint4*>(base + at * 2) = b;
+            *reinterpret_cast<uint2*>(base + (at + e0) * 2) = lo;
+            *reinterpret_cast<uint2*>(base + (at + e1) * 2) = hi;
         }
     }
 }
 
 template <int D, int XBF16>
-void launch(const AppendParams& p, cudaStream_t st) {
-    constexpr int H = 4;
-    const uint64_t items = (uint64_t)p.T * ((p.q_heads + 2 * p.kv.kv_heads + H - 1) / H);
-    const uint32_t per = kThreads / (D / 8);
-    attn_append_kernel<D, XBF16, H><<<(uint32_t)((items + per - 1) / per), kThreads, 0, st>>>(p);
+int launch(const AppendParams& p, int num_sms, cudaStream_t st) {
+    const uint32_t heads = p.q_heads + 2 * p.kv.kv_heads, per = kThreads / (D / 8);
+    const uint64_t four = ((uint64_t)p.T * ((heads + 3) / 4) + per - 1) / per;
+    const uint64_t two = ((uint64_t)p.T * ((heads + 1) / 2) + per - 1) / per;
+    if (two * per >= 0xffff0000u) return CZ_ESHAPE;  // (counted in 32 bits)
+    if (four >= 2 * (uint64_t)num_sms)
+        attn_append_kernel<D, XBF16, 4><<<(uint32_t)four, kThreads, 0, st>>>(p);
+    else
+        attn_append_kernel<D, XBF16, 2><<<(uint32_t)two, kThreads, 0, st>>>(p);
+    return cudaGetLastError() == cudaSuccess ? CZ_OK : CZ_ELAUNCH;
 }
 
 }  // namespace
 
-int attn_append_launch(const AppendParams& p, cudaStream_t st) {
-    if (p.kv.head_dim == 128)
-        p.x_bf16 ? launch<128, 1>(p, st) : launch<128, 0>(p, st);
-    else
-        p.x_bf16 ? launch<64, 1>(p, st) : launch<64, 0>(p, st);
-    return cudaGetLastError() == cudaSuccess ? CZ_OK : CZ_ELAUNCH;
+int attn_append_launch(const AppendParams& p, int num_sms, cudaStream_t st) {
+    if (p.kv.head_dim == 128) return p.x_bf16 ? launch<128, 1>(p, num_sms, st) : launch<128, 0>(p, num_sms, st);
+    return p.x_bf16 ? launch<64, 1>(p, num_sms, st) : launch<64, 0>(p, num_sms, st);
 }
 
 }  // namespace cz

@@ -235,7 +235,7 @@ struct AppendParams {
     uint16_t *q_out, *k_out, *v_out;  // bf16 bits; k_out, v_out nullable
     uint32_t* err;
 };
-int attn_append_launch(const AppendParams& p, cudaStream_t stream);
+int attn_append_launch(const AppendParams& p, int num_sms, cudaStream_t stream);
 
 struct AttnDecodeParams {
     KvView kv;
