@@ -14,8 +14,11 @@
 // tokens.  Keys and values are read once for all of them, a short prompt still fills
 // the tile (16 tokens of 8 heads), and the diagonal wastes at most 16 of 128 keys there.
 //
-// Warps: 0-3 and 4-7 softmax of query tile 0 and 1 (a thread a row), 8 TMA loads, 9 MMA
-// issue (10 and 11 lend their registers: 208 a thread for softmax, 88 for the rest).  Blocks take tiles from the largest key count down, so the last to finish are short.
+// One block per SM runs through pairs of query tiles, the longest first and in turn from either
+// end, so that the blocks end together; the next pair's queries, keys and first products go out
+// while the last one's results are written.  Warps: 0-3 and 4-7 softmax of query tile 0 and 1 (a
+// thread a row), 8 TMA loads, 9 MMA issue, 10 picks the pairs, 11 clears what lies behind the last
+// values.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -51,11 +54,16 @@ struct Cfg {
     static constexpr uint32_t OCOL = 256;              // O of tile i at OCOL + i * 128, S of tile i at i * 128
 };
 
+struct Pair {
+    int q0, nq, k0, nk, tile, head;  // sequence, pair of query tiles in it (tile < 0: no more), kv head and pass
+};
+
 struct Bars {
-    uint64_t qfull[2], full[8], empty[8], sfull[2], pready[2][2], odone[2], vask, vclean, drain;
+    uint64_t ifull[2], iempty[2];  // the picked pairs
+    uint64_t qfull[2], qfree[2], full[8], empty[8], sfull[2], pready[2][2], odone[2], vask, vclean, drain;
+    Pair pairs[2];
     uint32_t tmem;
     int abort, never;
-    int q0, nq, k0, nk, tile;  // this block's sequence and query tile pair (tile < 0: none)
 };
 
 __device__ __forceinline__ float ex2(float x) {
@@ -206,7 +214,7 @@ __device__ __forceinline__ int reach(int nq, int nk, int step, int x) {
 }
 
 // One warp: the query tile pair of rank `rank`, longest reach first.
-__device__ void pick(const AttnPrefillParams& p, int step, int rank, Bars& B) {
+__device__ __forceinline__ Pair pick(const AttnPrefillParams& p, int step, int rank) {
     const int lane = threadIdx.x & 31;
     auto count = [&](int x) {
         int c = 0;
@@ -269,14 +277,29 @@ __device__ void pick(const AttnPrefillParams& p, int step, int rank, Bars& B) {
             }
         }
     }
-    if (lane == 0) {
-        B.tile = tile;
-        B.q0 = q0;
-        B.nq = nq;
-        B.k0 = k0;
-        B.nk = nk;
-    }
+    return Pair{q0, nq, k0, nk, tile, 0};
 }
+
+// A pair's key tiles, per query tile: up to its last token's limit.
+struct Work {
+    int n0, n1, most, tok0, tok1;
+    // keys of the last tile that belong to the sequence; products past them are left out, and the rows that
+    // fill up the last 16 (a neighbour's, of any value) are cleared first
+    int last_keys;
+    bool unclean;
+
+    __device__ __forceinline__ Work(const Pair& w, int tokens) {
+        tok0 = w.tile * 2 * tokens;
+        tok1 = tok0 + tokens;
+        const int a = min(w.nq, tok0 + tokens) - 1 + w.nk - w.nq, b = min(w.nq, tok1 + tokens) - 1 + w.nk - w.nq;
+        n0 = tok0 >= w.nq || a < 0 ? 0 : a / kKeys + 1;
+        n1 = tok1 >= w.nq || b < 0 ? 0 : b / kKeys + 1;
+        most = max(n0, n1);
+        last_keys = most > 0 ? min(kKeys, w.nk - (most - 1) * kKeys) : 0;
+        unclean = last_keys & 15;
+    }
+    __device__ __forceinline__ int n(int i) const { return i ? n1 : n0; }
+};
 
 template <int D>
 __global__ void __launch_bounds__(kThreads, 1) attn_prefill_kernel(const __grid_constant__ PrefillArgs A) {
@@ -287,14 +310,12 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefill_kernel(const __grid_
     uint8_t* skv = sq + 2 * C::QBYTES;
     __shared__ Bars B;
     const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
-    const int heads = (int)p.kv_heads * A.htiles;
-    const int hi = (int)(blockIdx.x % heads), rank = (int)(blockIdx.x / heads);
-    const int kh = hi / A.htiles, head0 = (hi % A.htiles) * A.pack;  // first query head of the group's pass
-
-    if (warp == 0) pick(p, 2 * A.tokens, rank, B);
     if (warp == 8 && lane == 0) {
         for (int i = 0; i < 2; ++i) {
+            mbar_init(&B.ifull[i], 1);
+            mbar_init(&B.iempty[i], 11);  // loads, products, 8 softmax warps, the clearing warp
             mbar_init(&B.qfull[i], 1);
+            mbar_init(&B.qfree[i], 1);
             mbar_init(&B.sfull[i], 1);
             mbar_init(&B.pready[i][0], 4);
             mbar_init(&B.pready[i][1], 4);
@@ -324,192 +345,254 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefill_kernel(const __grid_
     fence_after();
     const uint32_t tmem = (uint32_t)uniform((int)B.tmem);
     volatile int* abort = &B.abort;
-    const int tile = uniform(B.tile), nq = uniform(B.nq), nk = uniform(B.nk), q0 = uniform(B.q0), k0 = uniform(B.k0);
-
-    // key tiles of each query tile: up to its last token's limit
-    int n[2], tok[2];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        tok[i] = tile * 2 * A.tokens + i * A.tokens;
-        const int last = min(nq, tok[i] + A.tokens) - 1 + nk - nq;
-        n[i] = tile < 0 || tok[i] >= nq || last < 0 ? 0 : last / kKeys + 1;
-    }
-    const int nmax = max(n[0], n[1]);
-    // keys of the last tile that belong to the sequence; products past them are left out, and the rows that
-    // fill up the last 16 (a neighbour's, of any value) are cleared first
-    const int last_keys = nmax > 0 ? min(kKeys, nk - (nmax - 1) * kKeys) : 0;
-    const bool unclean = last_keys & 15;
 
     auto gave_up = [&]() {
         *abort = 1;
         atomicOr(p.err, kAttnErrWait);
     };
+    // The t-th pair of this block, as the picking warp hands it out; false when there are no more.
+    auto next_pair = [&](int t, Pair& w) {
+        const int at = t & 1;
+        const bool ok = __all_sync(0xffffffffu, wait_bar(&B.ifull[at], (t >> 1) & 1, abort));
+        if (!ok) {
+            gave_up();
+            return false;
+        }
+        const Pair& x = B.pairs[at];
+        w.q0 = uniform(x.q0);
+        w.nq = uniform(x.nq);
+        w.k0 = uniform(x.k0);
+        w.nk = uniform(x.nk);
+        w.tile = uniform(x.tile);
+        w.head = uniform(x.head);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&B.iempty[at]);
+        return w.tile >= 0;
+    };
 
     // registers: 2 x 208 + 88 = 3 x 168, what the block was launched with
     if (warp >= 8) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
-      if (tile >= 0 && warp == 8) {
-        // ---------------- loads ----------------
-        if (lane == 0 && nmax > 0) {
+        if (warp == 8) {
+            // ---------------- loads ----------------
             const uint32_t qbytes = (uint32_t)(A.tokens * A.pack) * 128 * C::NX;
-            auto load_q = [&](int i) {
-                if (n[i] == 0) return;
-                mbar_arrive_expect_tx(&B.qfull[i], qbytes);
-#pragma unroll
-                for (int x = 0; x < C::NX; ++x)
-                    tma3d(smem_u32(sq + i * C::QBYTES + x * 128 * 128), &A.qmap, x * 64, kh * A.group + head0,
-                          q0 + tok[i], &B.qfull[i]);
-            };
-            int issued = 0;
-            auto load_kv = [&](const CUtensorMap* m, int j) {
-                const int s = issued % C::STAGES;
-                if (issued >= C::STAGES &&
-                    !wait_bar(&B.empty[s], ((issued / C::STAGES) & 1) ^ 1, abort)) {
-                    gave_up();
-                    return false;
-                }
-                mbar_arrive_expect_tx(&B.full[s], C::KVBYTES);
-#pragma unroll
-                for (int x = 0; x < C::NX; ++x)
-                    tma3d(smem_u32(skv + s * C::KVBYTES + x * kKeys * 128), m, x * 64, kh, k0 + j * kKeys, &B.full[s]);
-                ++issued;
-                return true;
-            };
-            load_q(0);
-            bool ok = load_kv(&A.kmap, 0);
-            load_q(1);
-            ok = ok && load_kv(&A.vmap, 0);
-            for (int j = 1; j < nmax && ok; ++j) ok = load_kv(&A.kmap, j) && load_kv(&A.vmap, j);
-            // no copy stays in flight behind the block's end (all have landed unless a wait gave up)
-            for (int i = max(0, issued - C::STAGES); i < issued; ++i)
-                if (!wait_bar(&B.full[i % C::STAGES], (i / C::STAGES) & 1, &B.never)) gave_up();
-        }
-        __syncwarp();
-      } else if (tile >= 0 && warp == 9) {
-        // ---------------- MMA ----------------
-        constexpr uint32_t IDS = idesc(128, kKeys, false), IDO = idesc(128, D, true);
-        const uint32_t tm = tmem;
-        const uint64_t dq = desc_k(smem_u32(sq)), dk = desc_k(smem_u32(skv));
-        const uint64_t dv = desc_mn(smem_u32(skv), kKeys * 128);
-        auto wait = [&](uint64_t* bar, uint32_t parity) {
-            const bool ok = __all_sync(0xffffffffu, wait_bar(bar, parity, abort));
-            if (!ok) gave_up();
-            return ok;
-        };
-        // the ring's uses in order: K_0, V_0, K_1, V_1, ...
-        int use = 0, ustage = 0;
-        uint32_t uphase = 0;
-        auto wait_kv = [&]() { return wait(&B.full[ustage], uphase); };
-        auto next_kv = [&]() {
-            const int st = ustage;
-            ++use;
-            if (++ustage == C::STAGES) ustage = 0, uphase ^= 1;
-            return st;
-        };
-        auto qk = [&](int i, int st) {  // S_i = Q_i K^T
-#pragma unroll
-            for (int k = 0; k < D / 16; ++k) {
-                const uint32_t off = (k / 4) * (128 * 128 / 16) + (k % 4) * 2;
-                mma_ss(tm + i * 128, dq + (uint32_t)(i * C::QBYTES / 16 + off), dk + (uint32_t)(st * C::KVBYTES / 16 + off),
-                       IDS, k > 0);
-            }
-            commit(&B.sfull[i]);
-        };
-        bool ok = nmax == 0 || wait_kv();
-        int kst = next_kv();
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-            if (ok && n[i] > 0) {
-                ok = wait(&B.qfull[i], 0);
-                if (ok) qk(i, kst);
-            }
-        if (ok && nmax > 0) commit(&B.empty[kst]);
+            int issued = 0, qused[2] = {0, 0};
+            bool ok = true;
+            Pair w;
 #pragma unroll 1
-        for (int j = 0; j < nmax && ok; ++j) {
-            const bool more = j + 1 < nmax;
-            const int ksteps = more ? kKeys / 16 : (last_keys + 15) / 16;
-            ok = wait_kv();
-            if (!ok) break;
-            bool ask = unclean && !more;
-            if (ask && lane == 0) mbar_arrive(&B.vask);
-            __syncwarp();
-            const int vst = next_kv();
-            bool kwait = more;
+            for (int t = 0; ok && next_pair(t, w); ++t) {
+                const Work k(w, A.tokens);
+                const int kh = w.head / A.htiles, head = kh * A.group + (w.head % A.htiles) * A.pack;
+                auto load_q = [&](int i) {
+                    if (k.n(i) == 0) return true;
+                    if (qused[i] && !wait_bar(&B.qfree[i], (qused[i] - 1) & 1, abort)) return false;
+                    ++qused[i];
+                    mbar_arrive_expect_tx(&B.qfull[i], qbytes);
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                if (j >= n[i] || !ok) continue;
-                auto pv = [&](int k) {
-                    if (k < ksteps)
-                        mma_ts(tm + C::OCOL + i * 128, tm + i * 128 + k * 8, dv + (uint32_t)((vst * C::KVBYTES + k * 2048) / 16),
-                               IDO, j > 0 || k > 0);
+                    for (int x = 0; x < C::NX; ++x)
+                        tma3d(smem_u32(sq + i * C::QBYTES + x * 128 * 128), &A.qmap, x * 64, head,
+                              w.q0 + (i ? k.tok1 : k.tok0), &B.qfull[i]);
+                    return true;
                 };
-                // the first 64 keys' products run under the other weights' exponentials
-                ok = wait(&B.pready[i][0], j & 1) && (!ask || wait(&B.vclean, 0));
-                if (!ok) continue;
-                ask = false;
-                fence_after();
+                auto load_kv = [&](const CUtensorMap* m, int j) {
+                    const int s = issued % C::STAGES;
+                    if (issued >= C::STAGES && !wait_bar(&B.empty[s], ((issued / C::STAGES) & 1) ^ 1, abort)) return false;
+                    mbar_arrive_expect_tx(&B.full[s], C::KVBYTES);
 #pragma unroll
-                for (int k = 0; k < 4; ++k) pv(k);
-                ok = wait(&B.pready[i][1], j & 1);
-                if (!ok) continue;
-                fence_after();
+                    for (int x = 0; x < C::NX; ++x)
+                        tma3d(smem_u32(skv + s * C::KVBYTES + x * kKeys * 128), m, x * 64, kh, w.k0 + j * kKeys, &B.full[s]);
+                    ++issued;
+                    return true;
+                };
+                if (k.most > 0 && lane == 0) {
+                    ok = load_kv(&A.kmap, 0) && load_q(0) && load_q(1) && load_kv(&A.vmap, 0);
+#pragma unroll 1
+                    for (int j = 1; j < k.most && ok; ++j) ok = load_kv(&A.kmap, j) && load_kv(&A.vmap, j);
+                    if (!ok) gave_up();
+                }
+                ok = uniform(ok);
+            }
+            // no copy stays in flight behind the block's end (all have landed unless a wait gave up)
+            if (lane == 0) {
+                for (int i = max(0, issued - C::STAGES); i < issued; ++i)
+                    if (!wait_bar(&B.full[i % C::STAGES], (i / C::STAGES) & 1, &B.never)) gave_up();
+                for (int i = 0; i < 2; ++i)
+                    if (qused[i] && !wait_bar(&B.qfull[i], (qused[i] - 1) & 1, &B.never)) gave_up();
+            }
+            __syncwarp();
+        } else if (warp == 9) {
+            // ---------------- products ----------------
+            constexpr uint32_t IDS = idesc(128, kKeys, false), IDO = idesc(128, D, true);
+            const uint64_t dq = desc_k(smem_u32(sq)), dk = desc_k(smem_u32(skv));
+            const uint64_t dv = desc_mn(smem_u32(skv), kKeys * 128);
+            auto wait = [&](uint64_t* bar, uint32_t parity) {
+                const bool ok = __all_sync(0xffffffffu, wait_bar(bar, parity, abort));
+                if (!ok) gave_up();
+                return ok;
+            };
+            // the ring's uses in order: K_0, V_0, K_1, V_1, ... of one pair after the other
+            int ustage = 0;
+            uint32_t uphase = 0, qphase[2] = {0, 0}, pphase[2] = {0, 0}, vphase = 0;
+            auto wait_kv = [&]() { return wait(&B.full[ustage], uphase); };
+            auto next_kv = [&]() {
+                const int st = ustage;
+                if (++ustage == C::STAGES) ustage = 0, uphase ^= 1;
+                return st;
+            };
+            auto qk = [&](int i, int st, bool last) {  // S_i = Q_i K^T
 #pragma unroll
-                for (int k = 4; k < 8; ++k) pv(k);
-                if (j + 1 == n[i]) {
-                    commit(&B.odone[i]);
-                } else {
-                    if (kwait) {
-                        ok = wait_kv();
-                        kst = next_kv();
-                        kwait = false;
+                for (int k = 0; k < D / 16; ++k) {
+                    const uint32_t off = (k / 4) * (128 * 128 / 16) + (k % 4) * 2;
+                    mma_ss(tmem + i * 128, dq + (uint32_t)(i * C::QBYTES / 16 + off),
+                           dk + (uint32_t)(st * C::KVBYTES / 16 + off), IDS, k > 0);
+                }
+                commit(&B.sfull[i]);
+                if (last) commit(&B.qfree[i]);
+            };
+            bool ok = true;
+            Pair w;
+#pragma unroll 1
+            for (int t = 0; ok && next_pair(t, w); ++t) {
+                const Work work(w, A.tokens);
+                if (work.most == 0) continue;
+                ok = wait_kv();
+                int kst = next_kv();
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+                    if (ok && work.n(i) > 0) {
+                        ok = wait(&B.qfull[i], qphase[i]);
+                        qphase[i] ^= 1;
+                        if (ok) qk(i, kst, work.n(i) == 1);
                     }
-                    if (ok) qk(i, kst);  // into S_i: in order behind the product that reads P_i from it
+                if (ok) commit(&B.empty[kst]);
+#pragma unroll 1
+                for (int j = 0; j < work.most && ok; ++j) {
+                    const bool more = j + 1 < work.most;
+                    const int ksteps = more ? kKeys / 16 : (work.last_keys + 15) / 16;
+                    ok = wait_kv();
+                    if (!ok) break;
+                    bool ask = work.unclean && !more;
+                    if (ask && lane == 0) mbar_arrive(&B.vask);
+                    __syncwarp();
+                    const int vst = next_kv();
+                    bool kwait = more;
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        if (j >= work.n(i) || !ok) continue;
+                        auto pv = [&](int k) {
+                            if (k < ksteps)
+                                mma_ts(tmem + C::OCOL + i * 128, tmem + i * 128 + k * 8,
+                                       dv + (uint32_t)((vst * C::KVBYTES + k * 2048) / 16), IDO, j > 0 || k > 0);
+                        };
+                        // the first 64 keys' products run under the other weights' exponentials
+                        ok = wait(&B.pready[i][0], pphase[i]) && (!ask || wait(&B.vclean, vphase));
+                        if (!ok) continue;
+                        if (ask) vphase ^= 1;
+                        ask = false;
+                        fence_after();
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) pv(k);
+                        ok = wait(&B.pready[i][1], pphase[i]);
+                        if (!ok) continue;
+                        pphase[i] ^= 1;
+                        fence_after();
+#pragma unroll
+                        for (int k = 4; k < 8; ++k) pv(k);
+                        if (j + 1 == work.n(i)) {
+                            commit(&B.odone[i]);
+                        } else {
+                            if (kwait) {
+                                ok = wait_kv();
+                                kst = next_kv();
+                                kwait = false;
+                            }
+                            // into S_i: in order behind the product that reads P_i from it
+                            if (ok) qk(i, kst, j + 2 == work.n(i));
+                        }
+                    }
+                    if (!ok) break;
+                    commit(&B.empty[vst]);
+                    if (more) commit(&B.empty[kst]);
                 }
             }
-            if (!ok) break;
-            commit(&B.empty[vst]);
-            if (more) commit(&B.empty[kst]);
-        }
-        // every product has finished before TMEM is given back
-        commit(&B.drain);
-        if (!wait_bar(&B.drain, 0, &B.never)) gave_up();
-        __syncwarp();
-      } else if (tile >= 0 && warp == 10 && unclean) {
-        // ---------------- the last values' tail ----------------
-        if (__all_sync(0xffffffffu, wait_bar(&B.vask, 0, abort))) {
-            uint8_t* v = skv + ((2 * nmax - 1) % C::STAGES) * C::KVBYTES;
-            for (int i = lane; i < (16 - (last_keys & 15)) * 8 * C::NX; i += 32) {
-                const int r = last_keys + i / (8 * C::NX), c = i % (8 * C::NX);
-                *reinterpret_cast<uint4*>(v + (c >> 3) * kKeys * 128 + r * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
-            }
-            fence_proxy_async_smem();
+            // every product has finished before TMEM is given back
+            commit(&B.drain);
+            if (!wait_bar(&B.drain, 0, &B.never)) gave_up();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&B.vclean);
+        } else if (warp == 10) {
+            // ---------------- the block's pairs, in turn from either end of each round ----------------
+            const int heads = (int)p.kv_heads * A.htiles;
+#pragma unroll 1
+            for (int t = 0;; ++t) {
+                const int at = t & 1;
+                if (t >= 2 && !__all_sync(0xffffffffu, wait_bar(&B.iempty[at], ((t >> 1) & 1) ^ 1, abort))) {
+                    gave_up();
+                    break;
+                }
+                const uint32_t item = t * gridDim.x + (t & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+                Pair w = pick(p, 2 * A.tokens, (int)(item / heads));
+                w.head = (int)(item % heads);
+                if (lane == 0) {
+                    B.pairs[at] = w;
+                    mbar_arrive(&B.ifull[at]);
+                }
+                if (w.tile < 0) break;
+            }
+        } else {
+            // ---------------- what lies behind the last values ----------------
+            int uses = 0;
+            uint32_t phase = 0;
+            Pair w;
+#pragma unroll 1
+            for (int t = 0; next_pair(t, w); ++t) {
+                const Work k(w, A.tokens);
+                uses += 2 * k.most;
+                if (!k.unclean) continue;
+                if (!__all_sync(0xffffffffu, wait_bar(&B.vask, phase, abort))) {
+                    gave_up();
+                    break;
+                }
+                phase ^= 1;
+                uint8_t* v = skv + ((uses - 1) % C::STAGES) * C::KVBYTES;
+                for (int i = lane; i < (16 - (k.last_keys & 15)) * 8 * C::NX; i += 32) {
+                    const int r = k.last_keys + i / (8 * C::NX), c = i % (8 * C::NX);
+                    *reinterpret_cast<uint4*>(v + (c >> 3) * kKeys * 128 + r * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
+                }
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&B.vclean);
+            }
         }
-      }
-    } else if (tile >= 0) {  // (the grid is sized without reading the bounds, and holds more blocks than query tiles)
+    } else {
         // ---------------- softmax: a thread a row ----------------
         asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
         const int i = warp >> 2;
         const int r = (warp & 3) * 32 + lane;
         const int lt = r / A.pack, lh = r % A.pack;
-        const int t = (i ? tok[1] : tok[0]) + lt;
-        const bool live = lt < A.tokens && t < nq && head0 + lh < A.group;
-        const int tiles = i ? n[1] : n[0];
-        const int lim0 = (i ? tok[1] : tok[0]) + nk - nq;  // the tile's first token's limit
-        const int lim = live ? t + nk - nq : 0x7fffffff;
         const uint32_t quad = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t sa = tmem + quad + i * 128, oa = tmem + quad + C::OCOL + i * 128;
         const float c = p.scale * 1.4426950408889634f;
-        float m = -INFINITY, l = 0.f;
+        uint32_t sphase = 0, ophase = 0;
         bool ok = true;
+        Pair w;
+#pragma unroll 1
+        for (int turn = 0; ok && next_pair(turn, w); ++turn) {
+        const Work work(w, A.tokens);
+        const int tok = i ? work.tok1 : work.tok0, tiles = work.n(i);
+        const int kh = w.head / A.htiles, head0 = (w.head % A.htiles) * A.pack;  // first query head of the group's pass
+        const int t = tok + lt;
+        const bool live = lt < A.tokens && t < w.nq && head0 + lh < A.group;
+        const int lim0 = tok + w.nk - w.nq;  // the tile's first token's limit
+        const int lim = live ? t + w.nk - w.nq : 0x7fffffff;
+        float m = -INFINITY, l = 0.f;
+#pragma unroll 1
         for (int j = 0; j < tiles; ++j) {
-            ok = wait_bar(&B.sfull[i], j & 1, abort);
-            if (!__all_sync(0xffffffffu, ok)) {
+            ok = __all_sync(0xffffffffu, wait_bar(&B.sfull[i], sphase, abort));
+            if (!ok) {
                 gave_up();
-                ok = false;
                 break;
             }
+            sphase ^= 1;
             fence_after();
             uint32_t sv[kKeys];
 #pragma unroll
@@ -575,17 +658,15 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefill_kernel(const __grid_
             l += e0 + e1;
         }
         if (ok && tiles > 0) {
-            ok = wait_bar(&B.odone[i], 0, abort);
-            if (!__all_sync(0xffffffffu, ok)) {
-                gave_up();
-                ok = false;
-            }
+            ok = __all_sync(0xffffffffu, wait_bar(&B.odone[i], ophase, abort));
+            if (!ok) gave_up();
+            ophase ^= 1;
             fence_after();
         }
         if (ok) {
             const float inv = m == -INFINITY ? 0.f : 1.f / l;  // no key seen: zeros
             uint4* dst = reinterpret_cast<uint4*>(
-                p.out + ((uint64_t)(q0 + t) * p.q_heads + (uint64_t)kh * A.group + head0 + lh) * D);
+                p.out + ((uint64_t)(w.q0 + t) * p.q_heads + (uint64_t)kh * A.group + head0 + lh) * D);
 #pragma unroll
             for (int x = 0; x < D / 32; ++x) {
                 uint32_t o[32];
@@ -596,19 +677,20 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefill_kernel(const __grid_
                 if (live) {
 #pragma unroll
                     for (int y = 0; y < 4; ++y) {
-                        uint32_t w[4];
+                        uint32_t v[4];
 #pragma unroll
                         for (int z = 0; z < 4; ++z)
-                            w[z] = inv == 0.f ? 0u
+                            v[z] = inv == 0.f ? 0u
                                               : pack_bf16(__uint_as_float(o[y * 8 + 2 * z]) * inv,
                                                           __uint_as_float(o[y * 8 + 2 * z + 1]) * inv);
-                        dst[x * 4 + y] = make_uint4(w[0], w[1], w[2], w[3]);
+                        dst[x * 4 + y] = make_uint4(v[0], v[1], v[2], v[3]);
                     }
                 }
                 __syncwarp();
             }
         }
-        fence_before();
+        fence_before();  // O is read before the next pair's weights are announced, and its products overwrite it
+        }
     }
     __syncthreads();
     if (warp == 9)
@@ -643,7 +725,7 @@ int launch(const PrefillArgs& a, uint32_t grid, cudaStream_t st) {
 
 }  // namespace
 
-int attn_prefill_launch(const AttnPrefillParams& p, int, cudaStream_t st) {
+int attn_prefill_launch(const AttnPrefillParams& p, int num_sms, cudaStream_t st) {
     if (p.Tk == 0)  // no query sees a key
         return cudaMemsetAsync(p.out, 0, (size_t)p.Tq * p.q_heads * p.head_dim * 2, st) == cudaSuccess ? CZ_OK
                                                                                                       : CZ_ELAUNCH;
@@ -653,13 +735,14 @@ int attn_prefill_launch(const AttnPrefillParams& p, int, cudaStream_t st) {
     a.htiles = (a.group + 127) / 128;
     a.pack = (a.group + a.htiles - 1) / a.htiles;
     a.tokens = 128 / a.pack;
-    const uint64_t grid = ((uint64_t)p.Tq / (2 * a.tokens) + p.B) * p.kv_heads * a.htiles;
-    if (grid > 0x7fffffffu) return CZ_ESHAPE;
+    const uint64_t pairs = ((uint64_t)p.Tq / (2 * a.tokens) + p.B) * p.kv_heads * a.htiles;  // at most
+    if (pairs > 0x3fffffffu) return CZ_ESHAPE;
+    const uint32_t grid = pairs < (uint64_t)num_sms ? (uint32_t)pairs : (uint32_t)num_sms;
     if (!make_map(&a.qmap, p.q, p.Tq, p.q_heads, p.head_dim, p.q_stride, a.pack, a.tokens) ||
         !make_map(&a.kmap, p.k, p.Tk, p.kv_heads, p.head_dim, p.k_stride, 1, kKeys) ||
         !make_map(&a.vmap, p.v, p.Tk, p.kv_heads, p.head_dim, p.v_stride, 1, kKeys))
         return CZ_ESHAPE;
-    return p.head_dim == 128 ? launch<128>(a, (uint32_t)grid, st) : launch<64>(a, (uint32_t)grid, st);
+    return p.head_dim == 128 ? launch<128>(a, grid, st) : launch<64>(a, grid, st);
 }
 
 }  // namespace cz
