@@ -49,8 +49,10 @@ struct Cfg {
     static constexpr int NX = D / 64;                  // 128-byte column blocks
     static constexpr int QBYTES = 128 * D * 2;
     static constexpr int KVBYTES = kKeys * D * 2;
-    static constexpr int STAGES = (227 * 1024 - 2048 - 2 * QBYTES) / KVBYTES > 8 ? 8 : (227 * 1024 - 2048 - 2 * QBYTES) / KVBYTES;
-    static constexpr int SMEM = 1024 + 2 * QBYTES + STAGES * KVBYTES;
+    static constexpr int OBYTES = 8 * 32 * 128;        // the epilogue's turning room: 64 columns of a warp's rows
+    static constexpr int ROOM = 227 * 1024 - 2048 - 2 * QBYTES - OBYTES;
+    static constexpr int STAGES = ROOM / KVBYTES > 8 ? 8 : ROOM / KVBYTES;
+    static constexpr int SMEM = 1024 + 2 * QBYTES + STAGES * KVBYTES + OBYTES;
     static constexpr uint32_t OCOL = 256;              // O of tile i at OCOL + i * 128, S of tile i at i * 128
 };
 
@@ -665,26 +667,39 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefill_kernel(const __grid_
         }
         if (ok) {
             const float inv = m == -INFINITY ? 0.f : 1.f / l;  // no key seen: zeros
-            uint4* dst = reinterpret_cast<uint4*>(
-                p.out + ((uint64_t)(w.q0 + t) * p.q_heads + (uint64_t)kh * A.group + head0 + lh) * D);
+            // A thread has a row, whose 16-byte pieces would go to 32 lines in one store: turned in shared
+            // memory (64 columns at a time, pieces swizzled by the row), a store covers four whole lines.
+            uint8_t* room = skv + C::STAGES * C::KVBYTES + warp * 32 * 128;
+            const unsigned long long row =
+                live ? ((unsigned long long)(w.q0 + t) * p.q_heads + (unsigned)(kh * A.group + head0 + lh)) * D : ~0ull;
 #pragma unroll
-            for (int x = 0; x < D / 32; ++x) {
-                uint32_t o[32];
-                if (tiles > 0) {
-                    ld32(o, oa + x * 32);
-                    wait_ld();
-                }
-                if (live) {
+            for (int x = 0; x < D / 64; ++x) {
 #pragma unroll
-                    for (int y = 0; y < 4; ++y) {
+                for (int y = 0; y < 2; ++y) {
+                    uint32_t o[32];
+                    if (tiles > 0) {
+                        ld32(o, oa + x * 64 + y * 32);
+                        wait_ld();
+                    }
+#pragma unroll
+                    for (int z = 0; z < 4; ++z) {
                         uint32_t v[4];
 #pragma unroll
-                        for (int z = 0; z < 4; ++z)
-                            v[z] = inv == 0.f ? 0u
-                                              : pack_bf16(__uint_as_float(o[y * 8 + 2 * z]) * inv,
-                                                          __uint_as_float(o[y * 8 + 2 * z + 1]) * inv);
-                        dst[x * 4 + y] = make_uint4(v[0], v[1], v[2], v[3]);
+                        for (int u = 0; u < 4; ++u)
+                            v[u] = inv == 0.f ? 0u
+                                              : pack_bf16(__uint_as_float(o[z * 8 + 2 * u]) * inv,
+                                                          __uint_as_float(o[z * 8 + 2 * u + 1]) * inv);
+                        *reinterpret_cast<uint4*>(room + lane * 128 + (((y * 4 + z) ^ (lane & 7)) << 4)) =
+                            make_uint4(v[0], v[1], v[2], v[3]);
                     }
+                }
+                __syncwarp();
+#pragma unroll
+                for (int y = 0; y < 8; ++y) {
+                    const int r4 = y * 4 + (lane >> 3), piece = lane & 7;
+                    const unsigned long long at = __shfl_sync(0xffffffffu, row, r4);
+                    const uint4 v = *reinterpret_cast<const uint4*>(room + r4 * 128 + ((piece ^ (r4 & 7)) << 4));
+                    if (at != ~0ull) *reinterpret_cast<uint4*>(p.out + at + x * 64 + piece * 8) = v;
                 }
                 __syncwarp();
             }
