@@ -37,7 +37,7 @@ constexpr int kStageBytes = 8192;  // keys, then values, of one step
 // With little work, an item of up to this many steps per warp stays in one block: the join over the
 // workspace costs more than the shorter loop gains.
 constexpr int kShort = 4;
-constexpr uint32_t kItemSteps = 2;  // what starting and ending an item costs a warp, in steps
+constexpr uint32_t kItemSteps = 3;  // what starting and ending an item costs a warp, in steps
 constexpr int kMaxTiles = 2;       // 8-head column tiles per pass
 constexpr int kSlotFloats = kMaxTiles * 8 * 128 + kMaxTiles * 8 * 2;  // o, then (m, l) per head
 
@@ -217,7 +217,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) attn_decode_kernel(const __gri
     __shared__ Rec recs[kWarps][2];
     __shared__ float2 stat[kWarps][2][NT * 8];  // (m, l)
     __shared__ int abort_flag, never;
-    __shared__ uint32_t last_flag;
+    __shared__ uint32_t last_flag[2];
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int g = lane >> 2, t4 = lane & 3;
@@ -761,20 +761,26 @@ __global__ void __launch_bounds__(kWarps * 32, 1) attn_decode_kernel(const __gri
             }
         }
     }
+    if (open_left < 0 && open_right < 0) return;
+    __syncthreads();  // the partials are written; then one release / acquire each
+    if (tid < 64 && lane == 0) {
+        const int x = tid ? open_right : open_left;
+        uint32_t last = 0;
+        if (x >= 0) {
+            const Rec& r = recs[x >> 1][x & 1];
+            const uint32_t c0 = r.start / bquota, c1 = (r.start + r.steps - 1) / bquota;
+            last = atom_add_acq_rel(A.counters + c0, 1u) == c1 - c0;
+            if (last) A.counters[c0] = 0;  // as found, for the next call
+        }
+        last_flag[tid >> 5] = last;
+    }
+    __syncthreads();
 #pragma unroll 1
     for (int side = 0; side < 2; ++side) {
+        if (!last_flag[side]) continue;
         const int x = side ? open_right : open_left;
-        if (x < 0) continue;
         const Rec& r = recs[x >> 1][x & 1];
         const uint32_t c0 = r.start / bquota, c1 = (r.start + r.steps - 1) / bquota;
-        __syncthreads();  // the partial is written; then one release / acquire by thread 0
-        if (tid == 0) {
-            const uint32_t arrived = atom_add_acq_rel(A.counters + c0, 1u);
-            last_flag = arrived == c1 - c0;
-            if (last_flag) A.counters[c0] = 0;  // as found, for the next call
-        }
-        __syncthreads();
-        if (!last_flag) continue;
         // the item's partials in order, a batch of loads in flight at a time (one at a time would cost a
         // trip to L2 each)
         constexpr int BATCH = 24;
@@ -791,7 +797,9 @@ __global__ void __launch_bounds__(kWarps * 32, 1) attn_decode_kernel(const __gri
                 float v[BATCH][EPT];
 #pragma unroll
                 for (int j = 0; j < BATCH; ++j) {
-                    const int q = min(c + j, parts - 1);
+                    ml[j] = make_float2(-INFINITY, 0.f);
+                    if (c + j >= parts) continue;
+                    const int q = c + j;
                     const float* x = A.slots + ((uint64_t)(c0 + q) * 2 + (q == 0 ? 1 : 0)) * kSlotFloats;
                     ml[j] = __ldcg(reinterpret_cast<const float2*>(x + kMaxTiles * 8 * 128) + h);
                     if (EPT == 4) {
@@ -804,7 +812,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) attn_decode_kernel(const __gri
                 }
                 float top = mm;
 #pragma unroll
-                for (int j = 0; j < BATCH; ++j) top = fmaxf(top, c + j < parts ? ml[j].x : -INFINITY);
+                for (int j = 0; j < BATCH; ++j) top = fmaxf(top, ml[j].x);
                 const float zz = top == -INFINITY ? 0.f : top, a = ex2(mm - zz);
                 mm = top;
                 ll *= a;
