@@ -39,6 +39,7 @@ constexpr int kStageBytes = 8192;  // keys, then values, of one step
 constexpr int kShort = 4;
 constexpr uint32_t kItemSteps = 3;  // what starting and ending an item costs a warp, in steps
 constexpr int kMaxTiles = 2;       // 8-head column tiles per pass
+constexpr int kBatch = 40;         // partials of other blocks joined at a time
 constexpr int kSlotFloats = kMaxTiles * 8 * 128 + kMaxTiles * 8 * 2;  // o, then (m, l) per head
 
 struct DecodeArgs {
@@ -99,6 +100,9 @@ __device__ __forceinline__ uint32_t cvt_e4m3x2(uint32_t two) {
     uint32_t h;
     asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"((uint16_t)two));
     return h;
+}
+__device__ __forceinline__ void cp_async16(void* dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
 }
 __device__ __forceinline__ uint32_t atom_add_acq_rel(uint32_t* p, uint32_t v) {
     uint32_t r;
@@ -704,11 +708,12 @@ __global__ void __launch_bounds__(kWarps * 32, 1) attn_decode_kernel(const __gri
 
     // ---- items cut between this block's warps, or between blocks ----
     __syncthreads();
-    constexpr int EPT = D / 32;  // a warp a head, 4 or 2 dims a lane
+    constexpr int EPT = 4;  // a warp a head, 4 dims a lane (half of the lanes for 64)
     const int jh = warp, jd = lane * EPT;
+    const bool on = jd < D;
     auto finish = [&](const Rec& r, int n, float* acc, float ll) {
         const int kh = r.item / (int)A.tiles, h = (r.item % (int)A.tiles) * NT * 8 + n * 8 + jh;
-        if (h >= (int)A.group) return;
+        if (h >= (int)A.group || !on) return;
         const float vscale = p.kv.v_scale ? __ldg(p.kv.v_scale + kh) : 1.f;
         const float f = ll > 0.f || ll != ll ? vscale / ll : 0.f;
         uint32_t* dst = reinterpret_cast<uint32_t*>(
@@ -744,7 +749,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) attn_decode_kernel(const __gri
 #pragma unroll
             for (int z = 0; z < 2 * kWarps; ++z) {
                 const float fz = __shfl_sync(0xffffffffu, f, z);
-                if (group >> z & 1) {
+                if ((group >> z & 1) && on) {
                     const float* v = reinterpret_cast<const float*>(z & 1 ? base + (z >> 1) * kStages * kStageBytes
                                                                           : base + C::RING + (z >> 1) * C::PART) +
                                      (n * 8 + jh) * C::JROW + jd;
@@ -756,7 +761,8 @@ __global__ void __launch_bounds__(kWarps * 32, 1) attn_decode_kernel(const __gri
                 finish(recs[x >> 1][x & 1], n, acc, ll);
             } else {
 #pragma unroll
-                for (int i = 0; i < EPT; ++i) slot[(n * 8 + jh) * D + jd + i] = acc[i];
+                for (int i = 0; i < EPT; ++i)
+                    if (on) slot[(n * 8 + jh) * D + jd + i] = acc[i];
                 if (jd == 0) *(reinterpret_cast<float2*>(slot + kMaxTiles * 8 * 128) + n * 8 + jh) = make_float2(mm, ll);
             }
         }
@@ -781,51 +787,45 @@ __global__ void __launch_bounds__(kWarps * 32, 1) attn_decode_kernel(const __gri
         const int x = side ? open_right : open_left;
         const Rec& r = recs[x >> 1][x & 1];
         const uint32_t c0 = r.start / bquota, c1 = (r.start + r.steps - 1) / bquota;
-        // the item's partials in order, a batch of loads in flight at a time (one at a time would cost a
-        // trip to L2 each)
-        constexpr int BATCH = 24;
+        // The item's partials in order.  Up to kBatch of them are fetched at once, each thread's own pieces into
+        // shared memory that is free by now (fetched one by one they would cost a trip to L2 each; held in
+        // registers, unrolled code that runs once and cold).
+        static_assert(kBatch * 8 * D * 4 <= C::RING + kWarps * C::PART, "a batch fits");
         const int parts = (int)(c1 - c0) + 1;
+        float* own = reinterpret_cast<float*>(base) + jh * D + jd;
 #pragma unroll 1
         for (int n = 0; n < NT; ++n) {
             const int h = n * 8 + jh;
             float acc[EPT], mm = -INFINITY, ll = 0.f;
 #pragma unroll
             for (int i = 0; i < EPT; ++i) acc[i] = 0.f;
+            auto part = [&](int q) { return A.slots + ((uint64_t)(c0 + q) * 2 + (q == 0 ? 1 : 0)) * kSlotFloats; };
+            auto stats = [&](int q) {
+                return q < parts ? __ldcg(reinterpret_cast<const float2*>(part(q) + kMaxTiles * 8 * 128) + h)
+                                 : make_float2(-INFINITY, 0.f);
+            };
 #pragma unroll 1
-            for (int c = 0; c < parts; c += BATCH) {
-                float2 ml[BATCH];
-                float v[BATCH][EPT];
-#pragma unroll
-                for (int j = 0; j < BATCH; ++j) {
-                    ml[j] = make_float2(-INFINITY, 0.f);
-                    if (c + j >= parts) continue;
-                    const int q = c + j;
-                    const float* x = A.slots + ((uint64_t)(c0 + q) * 2 + (q == 0 ? 1 : 0)) * kSlotFloats;
-                    ml[j] = __ldcg(reinterpret_cast<const float2*>(x + kMaxTiles * 8 * 128) + h);
-                    if (EPT == 4) {
-                        const float4 w = __ldcg(reinterpret_cast<const float4*>(x + h * D + jd));
-                        v[j][0] = w.x, v[j][1] = w.y, v[j][EPT - 2] = w.z, v[j][EPT - 1] = w.w;
-                    } else {
-                        const float2 w = __ldcg(reinterpret_cast<const float2*>(x + h * D + jd));
-                        v[j][0] = w.x, v[j][1] = w.y;
-                    }
-                }
-                float top = mm;
-#pragma unroll
-                for (int j = 0; j < BATCH; ++j) top = fmaxf(top, ml[j].x);
-                const float zz = top == -INFINITY ? 0.f : top, a = ex2(mm - zz);
+            for (int c = 0; c < parts; c += kBatch) {
+                const int cnt = min(kBatch, parts - c);
+#pragma unroll 1
+                for (int j = 0; on && j < cnt; ++j) cp_async16(own + j * 8 * D, part(c + j) + h * D + jd);
+                asm volatile("cp.async.commit_group;" ::: "memory");
+                // (m, l) of parts c + lane and c + 32 + lane
+                const float2 s0 = stats(c + lane), s1 = lane < kBatch - 32 ? stats(c + 32 + lane) : make_float2(-INFINITY, 0.f);
+                const float top = fmaxf(mm, warp_max(fmaxf(s0.x, s1.x))), zz = top == -INFINITY ? 0.f : top;
+                const float a = ex2(mm - zz), f0 = ex2(s0.x - zz), f1 = ex2(s1.x - zz);
                 mm = top;
-                ll *= a;
+                ll = __fmaf_rn(ll, a, warp_sum(__fmaf_rn(f0, s0.y, f1 * s1.y)));
 #pragma unroll
                 for (int i = 0; i < EPT; ++i) acc[i] *= a;
+                asm volatile("cp.async.wait_group 0;" ::: "memory");
+#pragma unroll 4
+                for (int j = 0; j < cnt; ++j) {
+                    const float f = __shfl_sync(0xffffffffu, j < 32 ? f0 : f1, j & 31);
+                    const float* v = own + j * 8 * D;
 #pragma unroll
-                for (int j = 0; j < BATCH; ++j) {
-                    if (c + j < parts) {
-                        const float f = ex2(ml[j].x - zz);
-                        ll = __fmaf_rn(f, ml[j].y, ll);
-#pragma unroll
-                        for (int i = 0; i < EPT; ++i) acc[i] = __fmaf_rn(f, v[j][i], acc[i]);
-                    }
+                    for (int i = 0; i < EPT; ++i)
+                        if (on) acc[i] = __fmaf_rn(f, v[i], acc[i]);
                 }
             }
             finish(r, n, acc, ll);

@@ -157,6 +157,38 @@ def test_decode_long_and_many(lens):
         assert torch.equal(plan.run(q, pg.table, pg.len_t), got)
 
 
+@pytest.mark.parametrize("hq,hk,d,page,e4m3", [(16, 2, 64, 16, True), (24, 2, 128, 48, False), (4, 4, 128, 16, True),
+                                               (6, 1, 64, 32, False)])
+def test_decode_many_ragged(hq, hk, d, page, e4m3):
+    """Hundreds of sequences, many empty or short, some cut between warps and blocks."""
+    g = gen(hq + page)
+    r = torch.Generator().manual_seed(page)
+    lens = [int(x) for x in (700 * torch.rand(400, generator=r) ** 4)]
+    lens[17] = 9000
+    lens[399] = 0
+    pg = Paged(g, lens, hk, d, page, e4m3)
+    q = randn(g, len(lens), hq, d, dtype=torch.bfloat16) * 2
+    plan = attn.DecodePlan(pg.cache, hq, len(lens))
+    got = plan.run(q, pg.table, pg.len_t)
+    close(got, *pg.want(q, d ** -0.5))
+    for _ in range(2):
+        assert torch.equal(plan.run(q, pg.table, pg.len_t), got)
+    attn.check()
+
+
+@pytest.mark.parametrize("hk,d,e4m3", [(1, 64, False), (1, 128, True), (2, 128, False)])
+def test_decode_one_item_over_all_blocks(hk, d, e4m3):
+    """Few pairs on a long cache: partials of up to all blocks joined, groups of 8 and of 16 heads."""
+    for hq in (8 * hk, 16 * hk):
+        g = gen(hk + d + hq)
+        pg = Paged(g, [50021], hk, d, 64, e4m3)
+        q = randn(g, 1, hq, d, dtype=torch.bfloat16) * 2
+        plan = attn.DecodePlan(pg.cache, hq, 1)
+        got = plan.run(q, pg.table, pg.len_t)
+        close(got, *pg.want(q, d ** -0.5))
+        assert torch.equal(plan.run(q, pg.table, pg.len_t), got)
+
+
 @pytest.mark.parametrize("e4m3", [False, True])
 @pytest.mark.parametrize("peak", [1e-3, 12.0, 60.0])
 def test_decode_flat_and_peaked_scores(peak, e4m3):
@@ -338,6 +370,19 @@ def test_prefill_of_nothing_and_of_no_keys():
     assert not attn.prefill(q, kv, kv, cu, cu0).any()
 
 
+def test_prefill_many_prompts():
+    """Several rounds of query tiles per block, more sequences than a warp has lanes."""
+    r = torch.Generator().manual_seed(1)
+    nq = [int(x) for x in 500 * torch.rand(150, generator=r) ** 3]
+    nk = [n + (37 * i % 300 if i % 4 == 0 else 0) for i, n in enumerate(nq)]
+    g = gen(8)
+    q, k, v, cu = prompts(g, nq, nk, 6, 2, 64, False)
+    got = attn.prefill(q, k, v, *cu)
+    close(got, *prefill_want(q, k, v, nq, nk, 64 ** -0.5))
+    assert torch.equal(attn.prefill(q, k, v, *cu), got)
+    attn.check()
+
+
 @pytest.mark.parametrize("n", [1024, 2500, 4099])
 def test_prefill_long_prompt(n):
     g = gen(n)
@@ -428,7 +473,8 @@ def within(got, want, size, step, floor=0.0):
 @pytest.mark.parametrize("hq,hk,d,rot,norm,T,page", [(32, 4, 128, 128, True, 1, 64), (32, 4, 128, 128, True, 77, 16),
                                                      (6, 2, 64, 64, False, 130, 48), (16, 16, 64, 32, True, 33, 128),
                                                      (5, 1, 128, 64, True, 50, 64), (7, 7, 128, 16, False, 9, 32),
-                                                     (4, 4, 64, 0, True, 20, 64), (64, 8, 128, 112, False, 300, 64)])
+                                                     (4, 4, 64, 0, True, 20, 64), (64, 8, 128, 112, False, 300, 64),
+                                                     (16, 16, 64, 64, True, 900, 32)])
 def test_append(hq, hk, d, rot, norm, T, page, x, e4m3):
     g = gen(T + hq)
     eps = 1e-5

@@ -36,7 +36,6 @@ def test_tokens_after_a_prompt_match_the_whole_prompt(cache):
     x = [torch.randn((k + 1, 256), generator=g) for k in n]
     whole = ex.Decoder(1, dims, 8, 2, 64, 16, 128, 3, dt)
     cut = ex.Decoder(1, dims, 8, 2, 64, 16, 128, 3, dt)
-    attended = []
     for dec in (whole, cut):  # the state behind the attention sublayer
         layer = dec.layers[0]
         layer.forward = lambda h, *a, _l=layer, **k: _l.attention(h, *a, **k)
@@ -49,7 +48,6 @@ def test_tokens_after_a_prompt_match_the_whole_prompt(cache):
     base = torch.stack([t[-1] for t in x]).cuda()  # the sublayer's own part
     rel = ((got - want).norm(dim=1) / (want - base).norm(dim=1)).max()
     assert float(rel) <= (2.0 ** -7 if cache == "bf16" else 2.0 ** -3), float(rel)
-    attended.append(got)
 
 
 def test_a_few_layers_and_tokens_run():
