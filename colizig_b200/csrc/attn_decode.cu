@@ -34,10 +34,13 @@ constexpr int kWarps = 8;
 // last blocks wait in (128 x 4,000 tokens: 171 us with 3, 163 us with 2).
 constexpr int kStages = 2;
 constexpr int kStageBytes = 8192;  // keys, then values, of one step
-// With little work, an item of up to this many steps per warp stays in one block: the join over the
-// workspace costs more than the shorter loop gains.
-constexpr int kShort = 4;
-constexpr uint32_t kItemSteps = 3;  // what starting and ending an item costs a warp, in steps
+// With little work, an item of up to this many steps per warp stays in one block: up to there the join over
+// the workspace costs more than the shorter loop gains (256 keys in bf16: 7.6 us in one block, 8.5 us in
+// two; 512 keys: 9.6 us in one, 8.8 us in four).
+constexpr int kShort = 2;
+// What starting and ending an item costs a warp, in steps (48 ragged sequences on E4M3: 34.1, 32.5, 31.8 and
+// 32.1 us with 1 to 4).
+constexpr uint32_t kItemSteps = 3;
 constexpr int kMaxTiles = 2;       // 8-head column tiles per pass
 constexpr int kBatch = 40;         // partials of other blocks joined at a time
 constexpr int kSlotFloats = kMaxTiles * 8 * 128 + kMaxTiles * 8 * 2;  // o, then (m, l) per head
@@ -887,7 +890,7 @@ int attn_decode_launch(const AttnDecodeParams& p, int num_sms, cudaStream_t st) 
     const bool two = a.group > 8;
     a.tiles = two ? (a.group + 15) / 16 : 1;
     // the line and its parts' ends are counted in 32 bits; a step is 16 keys or more
-    const uint64_t steps = (uint64_t)p.table_width * p.kv.page_size / 16 + kItemSteps + kWarps * kShort;
+    const uint64_t steps = (uint64_t)p.table_width * p.kv.page_size / 16 + kItemSteps + kWarps * 4;
     if ((uint64_t)p.B * p.kv.kv_heads * a.tiles * steps >= 0x7fff0000u) return CZ_ESHAPE;
     a.counters = reinterpret_cast<uint32_t*>(p.workspace);
     a.slots = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(p.workspace) + counter_bytes(num_sms));
