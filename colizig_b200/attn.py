@@ -34,9 +34,12 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 _F32, _BF16, _I32, _I64 = torch.float32, torch.bfloat16, torch.int32, torch.int64
 
 
-def _ready() -> None:
+def _ready(index: int) -> None:
+    """The library is up on the tensors' device (brought up there if it was not)."""
     if not gpu.available():
-        gpu.init()
+        gpu.init(index)
+    elif gpu.device() != index:
+        raise ValueError(f"tensors on cuda:{index}, the library runs on cuda:{gpu.device()}")
 
 
 def _current(index: int) -> int:
@@ -124,9 +127,9 @@ class KvCache:
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: Optional[torch.Tensor] = None,
                  v_scale: Optional[torch.Tensor] = None):
-        _ready()
         _need(k.is_cuda and k.dim() == 4 and k.shape == v.shape and k.device == v.device,
               "k and v must be CUDA tensors [pages, kv_heads, page_size, head_dim] of one shape")
+        _ready(k.get_device())
         _need(k.dtype == v.dtype and k.dtype in (torch.bfloat16, E4M3), "the cache is bf16 or float8_e4m3fn")
         pages, hk, page, d = k.shape
         _need(d in HEAD_DIMS, f"head_dim must be one of {HEAD_DIMS}, got {d}")
@@ -175,7 +178,7 @@ def append(cache: KvCache, q, k, v, positions, slots, rope=None, q_norm=None, k_
            packed: bool = False, q_out=None, k_out=None, v_out=None, stream=None):
     """Norm (when q_norm / k_norm f32 [head_dim] are given) and rotation (rope: ``rope_table``) of
     a step's projections q [T, q_heads, head_dim], k and v [T, kv_heads, head_dim] (f32 or bf16,
-    slices of a fused projection as they are); k and v go to cache row slots[t] (i64; page *
+    slices of a fused projection as they are; no output may overlap them); k and v go to cache row slots[t] (i64; page *
     page_size + row, negative: not cached, no slot twice), positions i32 [T].  Returns (q, k, v)
     packed in bf16; k and v (what ``prefill`` reads) are None unless packed or given."""
     dev, d, hk = cache._index, cache.head_dim, cache.kv_heads
@@ -265,11 +268,12 @@ def prefill(q, k, v, cu_q, cu_k=None, scale: Optional[float] = None, out=None, s
     """Causal attention over packed prompts: sequence b holds rows cu_q[b]..cu_q[b+1] of q
     [Tq, q_heads, head_dim] and cu_k[b]..cu_k[b+1] of k, v [Tk, kv_heads, head_dim] (bf16, row
     strides free; cu i32 [B + 1], cu_k defaults to cu_q).  Queries are the last tokens of
-    their sequence; a query that sees no key gives zeros.  scale defaults to head_dim ** -0.5."""
-    _ready()
+    their sequence; a query that sees no key gives zeros; rows past the last sequence's are not written.  scale
+    defaults to head_dim ** -0.5."""
     dev, d = q.get_device(), q.shape[-1]
     if dev < 0 or d not in HEAD_DIMS:
         raise ValueError(f"q must be a CUDA tensor of head_dim {HEAD_DIMS}, got {tuple(q.shape)} on {q.device}")
+    _ready(dev)
     Tq, hq, qs, qp = _rows("q", q, None, d, _BF16, dev)
     Tk, hk, ks, kp = _rows("k", k, None, d, _BF16, dev)
     tv, _, vs, vp = _rows("v", v, hk, d, _BF16, dev)

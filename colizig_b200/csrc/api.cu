@@ -36,6 +36,10 @@
 #include "cz_common.cuh"
 #include "cz_internal.h"
 
+namespace cz {
+uint32_t init_serial = 0;
+}
+
 #define CZ_EXPORT extern "C" __attribute__((visibility("default")))
 
 namespace {
@@ -516,6 +520,7 @@ int init_locked(int device) {
     }
     g.budget = 0;  // keyed store disabled until set (colizig_cuda.cu:184)
     g.inited = true;
+    ++cz::init_serial;
     return CZ_OK;
 }
 

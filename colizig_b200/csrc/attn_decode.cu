@@ -193,6 +193,10 @@ struct Cfg {
     static constexpr int NSUB = TS / 16;
     static constexpr int JROW = D + 4;
     static constexpr int RING = kWarps * kStages * kStageBytes;
+    // Weights go to f16 beside E4M3 values: 2^kShift above their maximum of 1, so that they stay normal down to
+    // 2^-28 of it and vanish under 2^-38 only (unshifted, a hundred thousand keys of weight 2^-25 each would be
+    // lost or doubled); bf16 has the range.  Partials are kept relative to 2^(m - kShift).
+    static constexpr float kShift = F8 ? 14.f : 0.f;
     // a warp's partial of the item it starts in; that of the item it ends in goes into its ring
     static constexpr int PART = NT * 8 * JROW * 4;
     static_assert(PART <= kStages * kStageBytes, "a partial fits the ring");
@@ -602,7 +606,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) attn_decode_kernel(const __gri
                     m[n][0] = mx[0];
                     m[n][1] = mx[1];
                 }
-                const float z0 = mx[0] == -INFINITY ? 0.f : mx[0], z1 = mx[1] == -INFINITY ? 0.f : mx[1];
+                const float z0 = mx[0] == -INFINITY ? 0.f : mx[0] - C::kShift, z1 = mx[1] == -INFINITY ? 0.f : mx[1] - C::kShift;
 #pragma unroll
                 for (int u = 0; u < C::NSUB; ++u) {
                     float e[4];
@@ -701,7 +705,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) attn_decode_kernel(const __gri
                 if (g == 0) {
 #pragma unroll
                     for (int i = 0; i < 2; ++i)
-                        stat[warp][which][n * 8 + 2 * t4 + i] = make_float2(m[n][i], l[n][i]);
+                        stat[warp][which][n * 8 + 2 * t4 + i] = make_float2(m[n][i] - C::kShift, l[n][i]);
                 }
             }
             if (lane == 0)
@@ -866,12 +870,12 @@ int launch(DecodeArgs& a, int grid, cudaStream_t st) {
     const size_t smem = 1024 + C::RING + (parts > prefix ? parts : prefix);
     constexpr size_t most = 227 * 1024 - 4096;  // beside the static variables
     if (smem > most) return CZ_ESHAPE;
-    static bool set = false;  // the library's lock is held
-    if (!set) {
+    static uint32_t set = 0;  // the library's lock is held
+    if (set != init_serial) {
         if (cudaFuncSetAttribute(attn_decode_kernel<D, F8, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                  (int)most) != cudaSuccess)
             return CZ_ELAUNCH;
-        set = true;
+        set = init_serial;
     }
     attn_decode_kernel<D, F8, NT><<<grid, kWarps * 32, smem, st>>>(a);
     return cudaGetLastError() == cudaSuccess ? CZ_OK : CZ_ELAUNCH;

@@ -191,6 +191,9 @@ int fp8_matmul_launch(float* y, const float* x, const uint8_t* w, const float* s
 
 // ---- attention over a paged key/value cache (attn_append.cu, attn_decode.cu, attn_prefill.cu) ----
 
+// Counts colizig_cuda_init calls that took effect (set-up per device is done again after each).
+extern uint32_t init_serial;
+
 // Attention error word.
 constexpr uint32_t kAttnErrIndex = 1u;  // an index in device memory was out of range (-11)
 constexpr uint32_t kAttnErrWait = 2u;   // a bounded wait gave up (-7)

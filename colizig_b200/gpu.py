@@ -16,18 +16,24 @@ import numpy as np
 from . import _abi
 
 _ready = False
+_device = 0
 
 
 def init(device: int = 0) -> None:
-    global _ready
+    global _ready, _device
     L = _abi.load()
     rc = L.colizig_cuda_init() if device == 0 else L.colizig_cuda_init_device(device)
     _abi.check("colizig_cuda_init", rc)
-    _ready = True
+    _ready, _device = True, device
 
 
 def available() -> bool:
     return _ready
+
+
+def device() -> int:
+    """Ordinal of the device the library was brought up on."""
+    return _device
 
 
 def deinit() -> None:

@@ -382,7 +382,8 @@ int colizig_cuda_attn_decode(const colizig_kv_cache* cache, const void* q, uint6
  * sequence's last tokens: query i sees the keys j <= i + nk - nq (nq, nk the
  * sequence's row counts), and gives zeros when there is none.  q [Tq, q_heads,
  * head_dim], k and v [Tk, kv_heads, head_dim] at the given row strides; cu_q, cu_k
- * int32 [B + 1], cu[0] = 0, ascending; out bf16 [Tq, q_heads, head_dim].  A key row
+ * int32 [B + 1], cu[0] = 0, ascending; out bf16 [Tq, q_heads, head_dim] (rows past
+ * cu_q[B] are not written).  A key row
  * must be finite where any query of its own sequence is computed; other sequences'
  * rows never reach a result.  0, -1, -8 (shape), -4. */
 int colizig_cuda_attn_prefill(const void* q, const void* k, const void* v, uint64_t q_stride, uint64_t k_stride,

@@ -218,6 +218,41 @@ def test_decode_huge_queries_on_e4m3(big):
     close(got, o, w)
 
 
+def test_decode_many_small_weights_on_e4m3():
+    """One key of score 17.3 among 200,000 of score 0, whose weights of 2^-25 sum up to the result."""
+    n, d = 200000, 128
+    cache = attn.KvCache.empty(n // 64, 1, 64, d, E4M3)
+    k = torch.zeros((n, d), device="cuda")
+    v = torch.ones((n, d), device="cuda")
+    k[777], v[777] = 1.0, 0.0
+    cache.k.copy_(k.view(-1, 1, 64, d).to(E4M3))
+    cache.v.copy_(v.view(-1, 1, 64, d).to(E4M3))
+    q = torch.ones((1, 8, d), device="cuda", dtype=torch.bfloat16)
+    scale = 17.3 / d
+    got = attn.DecodePlan(cache, 8, 1, scale=scale).run(
+        q, torch.arange(n // 64, dtype=torch.int32, device="cuda")[None], torch.tensor([n], dtype=torch.int32, device="cuda"))
+    o, w = softmax_rows(q[0], k, v, scale, torch.ones(8, n, dtype=torch.bool, device="cuda"))
+    assert 5e-3 < float(o[0, 0]) < 7e-3
+    close(got[0], o, w)
+
+
+def test_calls_work_after_shutdown_and_init():
+    """Set-up per device is done again after colizig_cuda_shutdown; the caller's buffers stay good."""
+    g = gen(50)
+    pg = Paged(g, [300, 20], 2, 128, 64)
+    q = randn(g, 2, 8, 128, dtype=torch.bfloat16)
+    plan = attn.DecodePlan(pg.cache, 8, 2)
+    want = plan.run(q, pg.table, pg.len_t)
+    pq, pk, pv, cu = prompts(g, [200], [200], 8, 2, 128, False)
+    wantp = attn.prefill(pq, pk, pv, cu[0])
+    torch.cuda.synchronize()
+    gpu.deinit()
+    gpu.init()
+    assert torch.equal(plan.run(q, pg.table, pg.len_t), want)
+    assert torch.equal(attn.prefill(pq, pk, pv, cu[0]), wantp)
+    attn.check()
+
+
 def test_decode_offsets_past_32_bits():
     """Pages whose first element lies past 2^32."""
     page, hk, d = 64, 1, 128
