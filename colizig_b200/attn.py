@@ -102,15 +102,10 @@ def _vector(name: str, t: Optional[torch.Tensor], n: int, index: int) -> Optiona
                      f"{tuple(shape)} on {t.device}")
 
 
-def _output(name: str, t: Optional[torch.Tensor], n: int, heads: int, dim: int, like: torch.Tensor, index: int):
-    """(t, its address), or a new tensor like `like` in bf16 when t is None."""
+def _output(name: str, t: Optional[torch.Tensor], n: int, heads: int, dim: int, bf16: torch.Tensor, index: int):
+    """(t, its address), or a new tensor when t is None (bf16: any bf16 tensor of the device)."""
     if t is None:
-        if like.dtype is not _BF16:
-            t = torch.empty((n, heads, dim), dtype=_BF16, device=like.device)
-        elif like.is_contiguous():
-            t = torch.empty_like(like)
-        else:
-            t = like.new_empty((n, heads, dim))
+        t = bf16.new_empty((n, heads, dim))
         return t, t.data_ptr()
     if t.dtype is not _BF16 or t.shape != (n, heads, dim) or t.get_device() != index or not t.is_contiguous() or \
             t.data_ptr() & 15:
@@ -151,6 +146,7 @@ class KvCache:
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
         self.pages, self.kv_heads, self.page_size, self.head_dim = pages, hk, page, d
         self.device, self._index = k.device, k.get_device()
+        self._bf16 = k if k.dtype is _BF16 else torch.empty(0, dtype=_BF16, device=k.device)
         self._c = _abi.KvCacheC(k.data_ptr(), v.data_ptr(), None if k_scale is None else k_scale.data_ptr(),
                                 None if v_scale is None else v_scale.data_ptr(), strides[0], strides[1], pages, page,
                                 hk, d, _abi.COLIZIG_KV_E4M3 if e4m3 else _abi.COLIZIG_KV_BF16)
@@ -203,11 +199,11 @@ def append(cache: KvCache, q, k, v, positions, slots, rope=None, q_norm=None, k_
         pp = _ints("positions", positions, T, _I32, dev)
     qn, kn = _vector("q_norm", q_norm, d, dev), _vector("k_norm", k_norm, d, dev)
     kop = vop = None
-    q_out, qop = _output("q_out", q_out, T, hq, d, q, dev)
+    q_out, qop = _output("q_out", q_out, T, hq, d, cache._bf16, dev)
     if packed or k_out is not None:
-        k_out, kop = _output("k_out", k_out, T, hk, d, k, dev)
+        k_out, kop = _output("k_out", k_out, T, hk, d, cache._bf16, dev)
     if packed or v_out is not None:
-        v_out, vop = _output("v_out", v_out, T, hk, d, v, dev)
+        v_out, vop = _output("v_out", v_out, T, hk, d, cache._bf16, dev)
     handle = _current(dev) if stream is None else _stream(stream, dev, (
         q, k, v, positions, slots, rope, q_norm, k_norm, cache.k, cache.v, cache.k_scale, cache.v_scale, q_out, k_out,
         v_out))

@@ -72,6 +72,7 @@ template <int D, int XBF16, int HEADS>
 __global__ void __launch_bounds__(kThreads, HEADS == 4 ? 8 : 10) attn_append_kernel(const AppendParams p) {
     constexpr int L = D / 8;
     const int sub = threadIdx.x % L;
+    pdl_wait();
     const uint32_t hq = p.q_heads, hk = p.kv.kv_heads;
     const uint32_t per_token = (hq + 2 * hk + HEADS - 1) / HEADS;  // groups of lanes
     const uint32_t item = blockIdx.x * (kThreads / L) + threadIdx.x / L;
@@ -182,11 +183,10 @@ int launch(const AppendParams& p, int num_sms, cudaStream_t st) {
     const uint64_t four = ((uint64_t)p.T * ((heads + 3) / 4) + per - 1) / per;
     const uint64_t two = ((uint64_t)p.T * ((heads + 1) / 2) + per - 1) / per;
     if (two * per >= 0xffff0000u) return CZ_ESHAPE;  // (counted in 32 bits)
-    if (four >= 2 * (uint64_t)num_sms)
-        attn_append_kernel<D, XBF16, 4><<<(uint32_t)four, kThreads, 0, st>>>(p);
-    else
-        attn_append_kernel<D, XBF16, 2><<<(uint32_t)two, kThreads, 0, st>>>(p);
-    return cudaGetLastError() == cudaSuccess ? CZ_OK : CZ_ELAUNCH;
+    const bool ok = four >= 2 * (uint64_t)num_sms
+                        ? launch_early(attn_append_kernel<D, XBF16, 4>, (uint32_t)four, kThreads, 0, st, p)
+                        : launch_early(attn_append_kernel<D, XBF16, 2>, (uint32_t)two, kThreads, 0, st, p);
+    return ok ? CZ_OK : CZ_ELAUNCH;
 }
 
 }  // namespace

@@ -245,6 +245,8 @@ __global__ void __launch_bounds__(kWarps * 32, 1) attn_decode_kernel(const __gri
         prefetch_tensormap(&A.vmap);
     }
 
+    pdl_wait();
+
     // ---- the line and this warp's part of it ----
     // of the sequences: steps and item costs; blocks with 1, 2 and 4 steps a warp; the longest
     Line line;
@@ -877,8 +879,7 @@ int launch(DecodeArgs& a, int grid, cudaStream_t st) {
             return CZ_ELAUNCH;
         set = init_serial;
     }
-    attn_decode_kernel<D, F8, NT><<<grid, kWarps * 32, smem, st>>>(a);
-    return cudaGetLastError() == cudaSuccess ? CZ_OK : CZ_ELAUNCH;
+    return launch_early(attn_decode_kernel<D, F8, NT>, grid, kWarps * 32, smem, st, a) ? CZ_OK : CZ_ELAUNCH;
 }
 
 }  // namespace

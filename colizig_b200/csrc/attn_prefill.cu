@@ -75,6 +75,9 @@ struct Bars {
     int abort, never;
 };
 
+// A value that is the same in every lane, as one the compiler knows to be.
+__device__ __forceinline__ int uniform(int x) { return __shfl_sync(0xffffffffu, x, 0); }
+
 __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -104,9 +107,6 @@ __host__ __device__ constexpr uint32_t idesc(int M, int N, bool bmn) {
     return (1u << 4) | (1u << 7) | (1u << 10) | (bmn ? 1u << 16 : 0u) | ((uint32_t)(N >> 3) << 17) |
            ((uint32_t)(M >> 4) << 24);
 }
-// A value that is the same in every lane, as one the compiler knows to be.
-__device__ __forceinline__ int uniform(int x) { return __shfl_sync(0xffffffffu, x, 0); }
-
 // The issuing warp runs converged and one elected lane issues: with warp-uniform operands the
 // descriptors stay in uniform registers (issued from a divergent branch, a product cost some 100 cycles
 // more than it took the tensor pipe).
@@ -222,29 +222,37 @@ __device__ __forceinline__ int reach(int nq, int nk, int step, int x) {
     return max(0, n - ((y + step - 1) / step - 1));
 }
 
-// One warp: the query tile pair of rank `rank`, longest reach first.
-__device__ __forceinline__ Pair pick(const AttnPrefillParams& p, int step, int rank) {
+// One warp: the query tile pair of rank `rank`, longest reach first.  own: this lane's sequence, kept by the
+// caller from pick to pick (the first 32; more are read again each time).
+struct Bounds {
+    int q0, nq, k0, nk;
+};
+__device__ __forceinline__ Pair pick(const AttnPrefillParams& p, int step, int rank, const Bounds& own) {
     const int lane = threadIdx.x & 31;
+    auto get = [&](int b, int& q0, int& nq, int& k0, int& nk) {
+        if (b < 32) q0 = own.q0, nq = own.nq, k0 = own.k0, nk = own.nk;
+        else bounds(p, b, q0, nq, k0, nk);
+    };
     auto count = [&](int x) {
         int c = 0;
+#pragma unroll 1
         for (int b = lane; b < p.B; b += 32) {
             int q0, nq, k0, nk;
-            bounds(p, b, q0, nq, k0, nk);
+            get(b, q0, nq, k0, nk);
             c += reach(nq, nk, step, x);
         }
         return (int)__reduce_add_sync(0xffffffffu, (unsigned)c);
     };
     int tile = -1, q0 = 0, nq = 0, k0 = 0, nk = 0;
     if (p.B == 1) {
-        const bool ok = bounds(p, 0, q0, nq, k0, nk);
-        if (!ok && rank == 0 && lane == 0) atomicOr(p.err, kAttnErrIndex);
+        q0 = uniform(own.q0), nq = uniform(own.nq), k0 = uniform(own.k0), nk = uniform(own.nk);
         const int n = (nq + step - 1) / step;
         tile = rank < n ? n - 1 - rank : -1;
     } else {
         int top = 0;  // past every reach
+#pragma unroll 1
         for (int b = lane; b < p.B; b += 32) {
-            const bool ok = bounds(p, b, q0, nq, k0, nk);
-            if (!ok && rank == 0) atomicOr(p.err, kAttnErrIndex);
+            get(b, q0, nq, k0, nk);
             top = max(top, nk + step);
         }
         top = (int)__reduce_max_sync(0xffffffffu, (unsigned)top) + 1;
@@ -261,7 +269,7 @@ __device__ __forceinline__ Pair pick(const AttnPrefillParams& p, int step, int r
                 int c = 0;
                 q0 = nq = k0 = nk = 0;
                 if (b < p.B) {
-                    bounds(p, b, q0, nq, k0, nk);
+                    get(b, q0, nq, k0, nk);
                     c = reach(nq, nk, step, lo) - reach(nq, nk, step, hi);
                 }
                 int inc = c;
@@ -350,6 +358,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefill_kernel(const __grid_
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
     fence_before();
+    pdl_wait();
     __syncthreads();
     fence_after();
     const uint32_t tmem = (uint32_t)uniform((int)B.tmem);
@@ -531,6 +540,14 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefill_kernel(const __grid_
         } else if (warp == 10) {
             // ---------------- the block's pairs, in turn from either end of each round ----------------
             const int heads = (int)p.kv_heads * A.htiles;
+            Bounds own = {0, 0, 0, 0};
+            if (lane < p.B && !bounds(p, lane, own.q0, own.nq, own.k0, own.nk)) atomicOr(p.err, kAttnErrIndex);
+            if (blockIdx.x == 0) {
+                Bounds x;
+#pragma unroll 1
+                for (int b = lane + 32; b < p.B; b += 32)
+                    if (!bounds(p, b, x.q0, x.nq, x.k0, x.nk)) atomicOr(p.err, kAttnErrIndex);
+            }
 #pragma unroll 1
             for (int t = 0;; ++t) {
                 const int at = t & 1;
@@ -539,7 +556,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefill_kernel(const __grid_
                     break;
                 }
                 const uint32_t item = t * gridDim.x + (t & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
-                Pair w = pick(p, 2 * A.tokens, (int)(item / heads));
+                Pair w = pick(p, 2 * A.tokens, (int)(item / heads), own);
                 w.head = (int)(item % heads);
                 if (lane == 0) {
                     B.pairs[at] = w;
@@ -741,8 +758,7 @@ int launch(const PrefillArgs& a, uint32_t grid, cudaStream_t st) {
             return CZ_ELAUNCH;
         set = init_serial;
     }
-    attn_prefill_kernel<D><<<grid, kThreads, Cfg<D>::SMEM, st>>>(a);
-    return cudaGetLastError() == cudaSuccess ? CZ_OK : CZ_ELAUNCH;
+    return launch_early(attn_prefill_kernel<D>, grid, kThreads, Cfg<D>::SMEM, st, a) ? CZ_OK : CZ_ELAUNCH;
 }
 
 }  // namespace

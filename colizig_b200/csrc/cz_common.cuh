@@ -264,6 +264,13 @@ static __device__ __noinline__ bool wait_geq_bounded(const uint32_t* p, uint32_t
     return false;
 }
 
+// ---- programmatic dependent launch ----------------------------------------
+// Every thread of a kernel launched early waits here, before its first access to global memory,
+// until the kernels before it have ended and their writes are visible.  (Blocks are set up as the
+// earlier kernel's end; letting them come sooner measured slower: 48 ragged sequences' decode 30.5 us
+// against 29.7, eleven packed prompts 57.5 against 52.5.)
+CZ_DEV void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 // ---- warp reductions ------------------------------------------------------
 CZ_DEV float warp_sum(float v) {
 #pragma unroll

@@ -194,6 +194,24 @@ int fp8_matmul_launch(float* y, const float* x, const uint8_t* w, const float* s
 // Counts colizig_cuda_init calls that took effect (set-up per device is done again after each).
 extern uint32_t init_serial;
 
+// Launch whose blocks may be set up while the kernel before them on the stream still runs (programmatic
+// dependent launch); the kernel waits for that one's end (pdl_wait) before it touches global memory.
+template <class... P, class... Q>
+inline bool launch_early(void (*kernel)(P...), uint32_t grid, uint32_t block, size_t smem, cudaStream_t st,
+                         const Q&... args) {
+    cudaLaunchAttribute at;
+    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t c = {};
+    c.gridDim = dim3(grid);
+    c.blockDim = dim3(block);
+    c.dynamicSmemBytes = smem;
+    c.stream = st;
+    c.attrs = &at;
+    c.numAttrs = 1;
+    return cudaLaunchKernelEx(&c, kernel, args...) == cudaSuccess;
+}
+
 // Attention error word.
 constexpr uint32_t kAttnErrIndex = 1u;  // an index in device memory was out of range (-11)
 constexpr uint32_t kAttnErrWait = 2u;   // a bounded wait gave up (-7)
