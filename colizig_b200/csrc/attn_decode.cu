@@ -220,7 +220,8 @@ __global__ void __launch_bounds__(kWarps * 32, 1) attn_decode_kernel(const __gri
     uint32_t* prefix = reinterpret_cast<uint32_t*>(base + C::RING);  // prologue: places before each sequence (one item's)
     __shared__ uint64_t full[kWarps][kStages];
     __shared__ uint32_t scan[kWarps][6];
-    // partials of the items a warp starts in (0) and ends in (1): item (-1: none), first and last of its keys here
+    // partials of the items a warp starts in (0) and ends in (1): item (-1: none), whether its first and its last
+    // keys are in it, place on the line and steps of the whole item
     struct Rec {
         int item, b, begins, ends;
         uint32_t start, steps;
@@ -255,7 +256,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) attn_decode_kernel(const __gri
     uint32_t sum[5] = {0, 0, 0, 0, 0};
     auto count = [&](int b) {
         const int l = seq_len(p, b);
-        if (blockIdx.x == 0 && warp == 0 && __ldg(p.lens + b) != l) atomicOr(p.err, kAttnErrIndex);
+        if (blockIdx.x == 0 && (warp == 0 || p.B > 32) && __ldg(p.lens + b) != l) atomicOr(p.err, kAttnErrIndex);
         const uint32_t n = (uint32_t)(l + C::TS - 1) / C::TS;
         sum[0] += n ? n + kItemSteps : 0;
         sum[1] += (n + kWarps - 1) / kWarps;

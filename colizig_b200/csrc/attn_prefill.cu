@@ -603,132 +603,132 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefill_kernel(const __grid_
         Pair w;
 #pragma unroll 1
         for (int turn = 0; ok && next_pair(turn, w); ++turn) {
-        const Work work(w, A.tokens);
-        const int tok = i ? work.tok1 : work.tok0, tiles = work.n(i);
-        const int kh = w.head / A.htiles, head0 = (w.head % A.htiles) * A.pack;  // first query head of the group's pass
-        const int t = tok + lt;
-        const bool live = lt < A.tokens && t < w.nq && head0 + lh < A.group;
-        const int lim0 = tok + w.nk - w.nq;  // the tile's first token's limit
-        const int lim = live ? t + w.nk - w.nq : 0x7fffffff;
-        float m = -INFINITY, l = 0.f;
+            const Work work(w, A.tokens);
+            const int tok = i ? work.tok1 : work.tok0, tiles = work.n(i);
+            const int kh = w.head / A.htiles, head0 = (w.head % A.htiles) * A.pack;  // first query head of the group's pass
+            const int t = tok + lt;
+            const bool live = lt < A.tokens && t < w.nq && head0 + lh < A.group;
+            const int lim0 = tok + w.nk - w.nq;  // the tile's first token's limit
+            const int lim = live ? t + w.nk - w.nq : 0x7fffffff;
+            float m = -INFINITY, l = 0.f;
 #pragma unroll 1
-        for (int j = 0; j < tiles; ++j) {
-            ok = __all_sync(0xffffffffu, wait_bar(&B.sfull[i], sphase, abort));
-            if (!ok) {
-                gave_up();
-                break;
-            }
-            sphase ^= 1;
-            fence_after();
-            uint32_t sv[kKeys];
+            for (int j = 0; j < tiles; ++j) {
+                ok = __all_sync(0xffffffffu, wait_bar(&B.sfull[i], sphase, abort));
+                if (!ok) {
+                    gave_up();
+                    break;
+                }
+                sphase ^= 1;
+                fence_after();
+                uint32_t sv[kKeys];
 #pragma unroll
-            for (int x = 0; x < 4; ++x) ld32(sv + x * 32, sa + x * 32);
-            wait_ld();
-            if (j * kKeys + kKeys - 1 > lim0) {
-                const int cut = lim - j * kKeys;  // columns past it are not seen
+                for (int x = 0; x < 4; ++x) ld32(sv + x * 32, sa + x * 32);
+                wait_ld();
+                if (j * kKeys + kKeys - 1 > lim0) {
+                    const int cut = lim - j * kKeys;  // columns past it are not seen
 #pragma unroll
-                for (int x = 0; x < kKeys; ++x)
-                    if (x > cut) sv[x] = 0xff800000u;
-            }
-            float mx[4] = {m, m, m, m};
+                    for (int x = 0; x < kKeys; ++x)
+                        if (x > cut) sv[x] = 0xff800000u;
+                }
+                float mx[4] = {m, m, m, m};
 #pragma unroll
-            for (int x = 0; x < kKeys; x += 8)
+                for (int x = 0; x < kKeys; x += 8)
 #pragma unroll
-                for (int y = 0; y < 4; ++y)
-                    mx[y] = max3(mx[y], __uint_as_float(sv[x + 2 * y]), __uint_as_float(sv[x + 2 * y + 1]));
-            const float top = max3(mx[0], mx[1], max3(mx[2], mx[2], mx[3]));
-            if (j == 0) {
-                m = top;
-            } else if (__any_sync(0xffffffffu, live && !((top - m) * c <= kSlack))) {
-                // the products into O behind this tile's S have finished: S's completion covers them
-                const float a = top == m ? 1.f : ex2((m - top) * c);
-                m = top;
-                l *= a;
+                    for (int y = 0; y < 4; ++y)
+                        mx[y] = max3(mx[y], __uint_as_float(sv[x + 2 * y]), __uint_as_float(sv[x + 2 * y + 1]));
+                const float top = max3(mx[0], mx[1], max3(mx[2], mx[2], mx[3]));
+                if (j == 0) {
+                    m = top;
+                } else if (__any_sync(0xffffffffu, live && !((top - m) * c <= kSlack))) {
+                    // the products into O behind this tile's S have finished: S's completion covers them
+                    const float a = top == m ? 1.f : ex2((m - top) * c);
+                    m = top;
+                    l *= a;
 #pragma unroll 1
-                for (int x = 0; x < D / 16; ++x) {
-                    uint32_t o[16];
-                    ld16(o, oa + x * 16);
-                    wait_ld();
-#pragma unroll
-                    for (int y = 0; y < 16; ++y) o[y] = __float_as_uint(__uint_as_float(o[y]) * a);
-                    st16(oa + x * 16, o);
-                }
-            }
-            const float mc = m == -INFINITY ? 0.f : m * c;
-            const f2 cc = pair(c, c), mm = pair(-mc, -mc);
-            f2 sum0 = 0, sum1 = 0;
-#pragma unroll
-            for (int x = 0; x < 4; ++x) {
-                uint32_t pk[16];
-#pragma unroll
-                for (int y = 0; y < 16; ++y) {
-                    const f2 t = fma2(pair(__uint_as_float(sv[x * 32 + 2 * y]), __uint_as_float(sv[x * 32 + 2 * y + 1])), cc, mm);
-                    float e0, e1;
-                    unpair(t, e0, e1);
-                    e0 = ex2(e0);
-                    e1 = ex2(e1);
-                    if (y & 1) sum1 = add2(sum1, pair(e0, e1));
-                    else sum0 = add2(sum0, pair(e0, e1));
-                    pk[y] = pack_bf16(e0, e1);  // the second product's operand; its sums stay in f32
-                }
-                st16(sa + x * 16, pk);  // over columns that are in registers by now
-                if (x & 1) {
-                    wait_st();
-                    fence_before();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&B.pready[i][x >> 1]);
-                }
-            }
-            float e0, e1;
-            unpair(add2(sum0, sum1), e0, e1);
-            l += e0 + e1;
-        }
-        if (ok && tiles > 0) {
-            ok = __all_sync(0xffffffffu, wait_bar(&B.odone[i], ophase, abort));
-            if (!ok) gave_up();
-            ophase ^= 1;
-            fence_after();
-        }
-        if (ok) {
-            const float inv = m == -INFINITY ? 0.f : 1.f / l;  // no key seen: zeros
-            // A thread has a row, whose 16-byte pieces would go to 32 lines in one store: turned in shared
-            // memory (64 columns at a time, pieces swizzled by the row), a store covers four whole lines.
-            uint8_t* room = skv + C::STAGES * C::KVBYTES + warp * 32 * 128;
-            const unsigned long long row =
-                live ? ((unsigned long long)(w.q0 + t) * p.q_heads + (unsigned)(kh * A.group + head0 + lh)) * D : ~0ull;
-#pragma unroll
-            for (int x = 0; x < D / 64; ++x) {
-#pragma unroll
-                for (int y = 0; y < 2; ++y) {
-                    uint32_t o[32];
-                    if (tiles > 0) {
-                        ld32(o, oa + x * 64 + y * 32);
+                    for (int x = 0; x < D / 16; ++x) {
+                        uint32_t o[16];
+                        ld16(o, oa + x * 16);
                         wait_ld();
-                    }
 #pragma unroll
-                    for (int z = 0; z < 4; ++z) {
-                        uint32_t v[4];
-#pragma unroll
-                        for (int u = 0; u < 4; ++u)
-                            v[u] = inv == 0.f ? 0u
-                                              : pack_bf16(__uint_as_float(o[z * 8 + 2 * u]) * inv,
-                                                          __uint_as_float(o[z * 8 + 2 * u + 1]) * inv);
-                        *reinterpret_cast<uint4*>(room + lane * 128 + (((y * 4 + z) ^ (lane & 7)) << 4)) =
-                            make_uint4(v[0], v[1], v[2], v[3]);
+                        for (int y = 0; y < 16; ++y) o[y] = __float_as_uint(__uint_as_float(o[y]) * a);
+                        st16(oa + x * 16, o);
                     }
                 }
-                __syncwarp();
+                const float mc = m == -INFINITY ? 0.f : m * c;
+                const f2 cc = pair(c, c), mm = pair(-mc, -mc);
+                f2 sum0 = 0, sum1 = 0;
 #pragma unroll
-                for (int y = 0; y < 8; ++y) {
-                    const int r4 = y * 4 + (lane >> 3), piece = lane & 7;
-                    const unsigned long long at = __shfl_sync(0xffffffffu, row, r4);
-                    const uint4 v = *reinterpret_cast<const uint4*>(room + r4 * 128 + ((piece ^ (r4 & 7)) << 4));
-                    if (at != ~0ull) *reinterpret_cast<uint4*>(p.out + at + x * 64 + piece * 8) = v;
+                for (int x = 0; x < 4; ++x) {
+                    uint32_t pk[16];
+#pragma unroll
+                    for (int y = 0; y < 16; ++y) {
+                        const f2 t = fma2(pair(__uint_as_float(sv[x * 32 + 2 * y]), __uint_as_float(sv[x * 32 + 2 * y + 1])), cc, mm);
+                        float e0, e1;
+                        unpair(t, e0, e1);
+                        e0 = ex2(e0);
+                        e1 = ex2(e1);
+                        if (y & 1) sum1 = add2(sum1, pair(e0, e1));
+                        else sum0 = add2(sum0, pair(e0, e1));
+                        pk[y] = pack_bf16(e0, e1);  // the second product's operand; its sums stay in f32
+                    }
+                    st16(sa + x * 16, pk);  // over columns that are in registers by now
+                    if (x & 1) {
+                        wait_st();
+                        fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&B.pready[i][x >> 1]);
+                    }
                 }
-                __syncwarp();
+                float e0, e1;
+                unpair(add2(sum0, sum1), e0, e1);
+                l += e0 + e1;
             }
-        }
-        fence_before();  // O is read before the next pair's weights are announced, and its products overwrite it
+            if (ok && tiles > 0) {
+                ok = __all_sync(0xffffffffu, wait_bar(&B.odone[i], ophase, abort));
+                if (!ok) gave_up();
+                ophase ^= 1;
+                fence_after();
+            }
+            if (ok) {
+                const float inv = m == -INFINITY ? 0.f : 1.f / l;  // no key seen: zeros
+                // A thread has a row, whose 16-byte pieces would go to 32 lines in one store: turned in shared
+                // memory (64 columns at a time, pieces swizzled by the row), a store covers four whole lines.
+                uint8_t* room = skv + C::STAGES * C::KVBYTES + warp * 32 * 128;
+                const unsigned long long row =
+                    live ? ((unsigned long long)(w.q0 + t) * p.q_heads + (unsigned)(kh * A.group + head0 + lh)) * D : ~0ull;
+#pragma unroll
+                for (int x = 0; x < D / 64; ++x) {
+#pragma unroll
+                    for (int y = 0; y < 2; ++y) {
+                        uint32_t o[32];
+                        if (tiles > 0) {
+                            ld32(o, oa + x * 64 + y * 32);
+                            wait_ld();
+                        }
+#pragma unroll
+                        for (int z = 0; z < 4; ++z) {
+                            uint32_t v[4];
+#pragma unroll
+                            for (int u = 0; u < 4; ++u)
+                                v[u] = inv == 0.f ? 0u
+                                                  : pack_bf16(__uint_as_float(o[z * 8 + 2 * u]) * inv,
+                                                              __uint_as_float(o[z * 8 + 2 * u + 1]) * inv);
+                            *reinterpret_cast<uint4*>(room + lane * 128 + (((y * 4 + z) ^ (lane & 7)) << 4)) =
+                                make_uint4(v[0], v[1], v[2], v[3]);
+                        }
+                    }
+                    __syncwarp();
+#pragma unroll
+                    for (int y = 0; y < 8; ++y) {
+                        const int r4 = y * 4 + (lane >> 3), piece = lane & 7;
+                        const unsigned long long at = __shfl_sync(0xffffffffu, row, r4);
+                        const uint4 v = *reinterpret_cast<const uint4*>(room + r4 * 128 + ((piece ^ (r4 & 7)) << 4));
+                        if (at != ~0ull) *reinterpret_cast<uint4*>(p.out + at + x * 64 + piece * 8) = v;
+                    }
+                    __syncwarp();
+                }
+            }
+            fence_before();  // O is read before the next pair's weights are announced, and its products overwrite it
         }
     }
     __syncthreads();

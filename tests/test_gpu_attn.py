@@ -308,6 +308,44 @@ def test_decode_bad_indices_are_reported_and_not_followed():
     attn.check()
 
 
+@pytest.mark.parametrize("at", [0, 33, 150, 199])
+def test_decode_bad_length_in_a_large_batch(at):
+    g = gen(60)
+    pg = Paged(g, [5 + i % 40 for i in range(200)], 1, 64, 16)
+    q = randn(g, 200, 2, 64, dtype=torch.bfloat16)
+    plan = attn.DecodePlan(pg.cache, 2, 200)
+    good = plan.run(q, pg.table, pg.len_t)
+    attn.check()
+    for bad in (-3, pg.width * 16 + 1):
+        lens = pg.len_t.clone()
+        lens[at] = bad
+        got = plan.run(q, pg.table.clamp(min=0), lens)
+        keep = torch.arange(200, device="cuda") != at
+        assert torch.equal(got[keep], good[keep])
+        with pytest.raises(ColizigError) as e:
+            attn.check()
+        assert e.value.rc == -11
+
+
+def test_prefill_bad_bounds_among_many_are_reported():
+    g = gen(61)
+    n = [3 + i % 20 for i in range(90)]
+    q, k, v, cu = prompts(g, n, n, 4, 2, 64, False)
+    good = attn.prefill(q, k, v, cu[0])
+    attn.check()
+    for at in (1, 40, 90):
+        bad = cu[1].clone()
+        bad[at] = k.shape[0] + 7
+        got = attn.prefill(q, k, v, cu[0], bad)
+        rows = torch.ones(q.shape[0], dtype=torch.bool, device="cuda")
+        ends = cu[0].tolist()
+        rows[ends[at - 1]: ends[min(at + 1, 90)]] = False  # the sequences that name the bad bound
+        assert torch.equal(got[rows], good[rows])
+        with pytest.raises(ColizigError) as e:
+            attn.check()
+        assert e.value.rc == -11
+
+
 def test_decode_in_a_graph_follows_lengths():
     """Lengths and tables are read on the device: one captured step serves a growing cache."""
     g = gen(5)
