@@ -11,8 +11,10 @@ projections (src/qwen3moe/attn.zig:46-78 keys q/k/v/o; the projections themselve
 
 Tensors are torch CUDA tensors on the library's device; every call is queued on `stream`
 (default: torch's current stream), allocates outputs only when they are not given, and can
-be captured into a CUDA graph.  Given another stream than the current one, a call marks the
-tensors it takes as used there, so that their memory is not handed out while it runs.
+be captured into a CUDA graph.  Given another stream than the current one, a call allocates its
+outputs there and marks the tensors it takes as used there, so that their memory is not handed
+out while it runs.  Tensors that do not fit raise ValueError before anything is queued (the
+checks are native code, csrc/attn_binding.cpp).
 """
 
 from __future__ import annotations
@@ -28,10 +30,23 @@ HEAD_DIMS = (64, 128)
 E4M3 = torch.float8_e4m3fn
 
 
-# A decode step is a few microseconds on the device: the checks below read each attribute
-# once and build messages only when something is wrong.
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
-_F32, _BF16, _I32, _I64 = torch.float32, torch.bfloat16, torch.int32, torch.int64
+_bound = None
+
+
+def _native():
+    """The native binding, given the library's entry points."""
+    global _bound
+    if _bound is None:
+        try:
+            from . import _attn_native as m
+        except ImportError as e:
+            raise RuntimeError("colizig_b200/_attn_native.so is missing: build it with __graft_entry__.build()") from e
+        L = _abi.load()
+        m.bind(*(ctypes.cast(f, ctypes.c_void_p).value for f in
+                 (L.colizig_cuda_attn_append, L.colizig_cuda_attn_decode, L.colizig_cuda_attn_prefill)))
+        _bound = m
+    return _bound
 
 
 def _ready(index: int) -> None:
@@ -47,71 +62,31 @@ def _current(index: int) -> int:
     return _raw_stream(index) if _raw_stream is not None else torch.cuda.current_stream(index).cuda_stream
 
 
-def _stream(stream, index: int, tensors) -> int:
-    """The stream's handle; tensors used on another stream than the current one are marked."""
+def _elsewhere(stream, index: int):
+    """(handle, torch stream) of a given stream; the torch stream is None when it is the current one."""
     handle = getattr(stream, "cuda_stream", stream)
-    if handle != _current(index):
-        s = stream if isinstance(stream, torch.cuda.Stream) else torch.cuda.ExternalStream(handle, device=index)
-        for t in tensors:
-            if t is not None:
-                t.record_stream(s)
-    return handle
+    if handle == _current(index):
+        return handle, None
+    return handle, stream if isinstance(stream, torch.cuda.Stream) else torch.cuda.ExternalStream(handle, device=index)
+
+
+def _mark(s, *tensors) -> None:
+    for t in tensors:
+        if isinstance(t, torch.Tensor) and t.is_cuda:
+            t.record_stream(s)
+
+
+def _room(s, t: Optional[torch.Tensor], shape, device):
+    """An output for work on stream s: given, or allocated there."""
+    if t is not None:
+        return t
+    with torch.cuda.stream(s):
+        return torch.empty(shape, dtype=torch.bfloat16, device=device)
 
 
 def _need(ok: bool, what: str) -> None:
     if not ok:
         raise ValueError(what)
-
-
-def _rows(name: str, t: torch.Tensor, heads: Optional[int], dim: int, dtype, index: int):
-    """Checks [rows, heads, dim] with packed heads and any 16-byte aligned row stride; returns
-    (rows, heads, row stride in elements, address)."""
-    shape = t.shape
-    if len(shape) == 3 and t.dtype is dtype and t.get_device() == index:
-        n, h, d = shape
-        s0, s1, s2 = t.stride()
-        if d == dim and (h == heads or heads is None) and s2 == 1 and (s1 == dim or h <= 1):
-            at = t.data_ptr()
-            if n <= 1:
-                s0 = h * dim  # one row (or none): its stride is never used
-            if s0 >= h * dim and not (s0 * (4 if dtype is _F32 else 2) | at) & 15:
-                return n, h, s0, at
-            raise ValueError(f"{name}: rows must be 16-byte aligned and must not overlap")
-    raise ValueError(f"{name} must be {dtype} [rows, {heads if heads is not None else 'heads'}, {dim}] with packed heads "
-                     f"on cuda:{index}, got {t.dtype} {tuple(shape)} (strides {t.stride()}) on {t.device}")
-
-
-def _ints(name: str, t: torch.Tensor, n: int, dtype, index: int) -> int:
-    shape = t.shape
-    if len(shape) == 1 and shape[0] == n and t.dtype is dtype and t.get_device() == index and \
-            (n <= 1 or t.stride(0) == 1):
-        return t.data_ptr()
-    raise ValueError(f"{name} must be a packed {dtype} tensor [{n}] on cuda:{index}, got {t.dtype} {tuple(shape)} on "
-                     f"{t.device}")
-
-
-def _vector(name: str, t: Optional[torch.Tensor], n: int, index: int) -> Optional[int]:
-    if t is None:
-        return None
-    shape = t.shape
-    if len(shape) == 1 and shape[0] == n and t.dtype is _F32 and t.get_device() == index and t.stride(0) == 1:
-        at = t.data_ptr()
-        if not at & 15:
-            return at
-    raise ValueError(f"{name} must be a packed, 16-byte aligned f32 [{n}] tensor on cuda:{index}, got {t.dtype} "
-                     f"{tuple(shape)} on {t.device}")
-
-
-def _output(name: str, t: Optional[torch.Tensor], n: int, heads: int, dim: int, bf16: torch.Tensor, index: int):
-    """(t, its address), or a new tensor when t is None (bf16: any bf16 tensor of the device)."""
-    if t is None:
-        t = bf16.new_empty((n, heads, dim))
-        return t, t.data_ptr()
-    if t.dtype is not _BF16 or t.shape != (n, heads, dim) or t.get_device() != index or not t.is_contiguous() or \
-            t.data_ptr() & 15:
-        raise ValueError(f"{name} must be a contiguous, 16-byte aligned bf16 tensor {(n, heads, dim)} on cuda:{index}, "
-                         f"got {t.dtype} {tuple(t.shape)} on {t.device}")
-    return t, t.data_ptr()
 
 
 class KvCache:
@@ -146,11 +121,11 @@ class KvCache:
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
         self.pages, self.kv_heads, self.page_size, self.head_dim = pages, hk, page, d
         self.device, self._index = k.device, k.get_device()
-        self._bf16 = k if k.dtype is _BF16 else torch.empty(0, dtype=_BF16, device=k.device)
         self._c = _abi.KvCacheC(k.data_ptr(), v.data_ptr(), None if k_scale is None else k_scale.data_ptr(),
                                 None if v_scale is None else v_scale.data_ptr(), strides[0], strides[1], pages, page,
                                 hk, d, _abi.COLIZIG_KV_E4M3 if e4m3 else _abi.COLIZIG_KV_BF16)
-        self._ref = ctypes.byref(self._c)
+        self._at = ctypes.addressof(self._c)
+        self._lib = _native()
 
     @staticmethod
     def empty(pages: int, kv_heads: int, page_size: int, head_dim: int, dtype=torch.bfloat16, device="cuda",
@@ -177,41 +152,22 @@ def append(cache: KvCache, q, k, v, positions, slots, rope=None, q_norm=None, k_
     slices of a fused projection as they are; no output may overlap them); k and v go to cache row slots[t] (i64; page *
     page_size + row, negative: not cached, no slot twice), positions i32 [T].  Returns (q, k, v)
     packed in bf16; k and v (what ``prefill`` reads) are None unless packed or given."""
-    dev, d, hk = cache._index, cache.head_dim, cache.kv_heads
-    dt = _F32 if q.dtype is _F32 else _BF16
-    T, hq, qs, qp = _rows("q", q, None, d, dt, dev)
-    if hq < 1 or hq % hk:
-        raise ValueError(f"{hq} query heads are not a multiple of {hk} key/value heads")
-    tk, _, ks, kp = _rows("k", k, hk, d, dt, dev)
-    tv, _, vs, vp = _rows("v", v, hk, d, dt, dev)
-    if tk != T or tv != T:
-        raise ValueError("q, k and v must hold the same tokens")
-    sp = _ints("slots", slots, T, _I64, dev)
-    rp, rlen, rot, pp = None, 0, 0, None
-    if rope is not None:
-        shape = rope.shape
-        if len(shape) != 2 or rope.dtype is not _F32 or rope.get_device() != dev or not rope.is_contiguous() or \
-                rope.data_ptr() & 15 or shape[1] % 16 or not 0 < shape[1] <= d or shape[0] < 1:
-            raise ValueError(f"rope must be a contiguous f32 [positions, rot_dim] table on cuda:{dev}, rot_dim a "
-                             f"multiple of 16 up to {d}")
-        rlen, rot = shape
-        rp = rope.data_ptr()
-        pp = _ints("positions", positions, T, _I32, dev)
-    qn, kn = _vector("q_norm", q_norm, d, dev), _vector("k_norm", k_norm, d, dev)
-    kop = vop = None
-    q_out, qop = _output("q_out", q_out, T, hq, d, cache._bf16, dev)
-    if packed or k_out is not None:
-        k_out, kop = _output("k_out", k_out, T, hk, d, cache._bf16, dev)
-    if packed or v_out is not None:
-        v_out, vop = _output("v_out", v_out, T, hk, d, cache._bf16, dev)
-    handle = _current(dev) if stream is None else _stream(stream, dev, (
-        q, k, v, positions, slots, rope, q_norm, k_norm, cache.k, cache.v, cache.k_scale, cache.v_scale, q_out, k_out,
-        v_out))
-    rc = _abi.load().colizig_cuda_attn_append(cache._ref, qp, kp, vp, 0 if dt is _F32 else 1, T, hq, qs, ks, vs, pp, sp,
-                                              rp, rlen, rot, qn, kn, eps, qop, kop, vop, handle)
-    if rc:
-        _abi.check("colizig_cuda_attn_append", rc)
-    return q_out, k_out, v_out
+    dev = cache._index
+    if stream is None:
+        handle = _current(dev)
+    else:
+        handle, s = _elsewhere(stream, dev)
+        if s is not None:
+            _mark(s, q, k, v, positions, slots, rope, q_norm, k_norm, cache.k, cache.v, cache.k_scale, cache.v_scale, q_out,
+                  k_out, v_out)
+            q_out = _room(s, q_out, q.shape, cache.device)
+            k_out = _room(s, k_out, k.shape, cache.device) if packed else k_out
+            v_out = _room(s, v_out, v.shape, cache.device) if packed else v_out
+    r = cache._lib.append(cache._at, dev, q, k, v, positions, slots, rope, q_norm, k_norm, eps, packed, q_out, k_out, v_out,
+                          handle)
+    if r.__class__ is int:
+        _abi.check("colizig_cuda_attn_append", r)
+    return r
 
 
 class DecodePlan:
@@ -226,38 +182,27 @@ class DecodePlan:
         _need(1 <= max_batch <= _abi.COLIZIG_ATTN_MAX_BATCH, f"max_batch must be 1..{_abi.COLIZIG_ATTN_MAX_BATCH}")
         self.cache, self.q_heads, self.max_batch = cache, q_heads, max_batch
         self.scale = cache.head_dim ** -0.5 if scale is None else float(scale)
-        L = _abi.load()
-        self._fn = L.colizig_cuda_attn_decode
         with torch.cuda.device(cache.device):
-            self._ws = torch.zeros(L.colizig_cuda_attn_decode_workspace(), dtype=torch.uint8, device=cache.device)
+            self._ws = torch.zeros(_abi.load().colizig_cuda_attn_decode_workspace(), dtype=torch.uint8,
+                                   device=cache.device)
         self._wsp = self._ws.data_ptr()
 
     def run(self, q, table, lens, out=None, stream=None):
         """out [B, q_heads, head_dim] bf16 = attention of q (bf16, row stride free) over the lens[b]
         first tokens of the pages table[b] (i32 [B, width], row stride free; lens i32 [B])."""
         c = self.cache
-        dev, d, hq = c._index, c.head_dim, self.q_heads
-        B, _, qs, qp = _rows("q", q, hq, d, _BF16, dev)
-        if B > self.max_batch:
-            raise ValueError(f"{B} sequences, the plan holds {self.max_batch}")
-        shape = table.shape
-        if len(shape) != 2 or shape[0] != B or shape[1] < 1 or table.dtype is not _I32 or table.get_device() != dev:
-            raise ValueError(f"table must be an i32 tensor [{B}, width] on cuda:{dev}, got {table.dtype} {tuple(shape)} "
-                             f"on {table.device}")
-        width = shape[1]
-        t0, t1 = table.stride()
-        if B <= 1:
-            t0 = width
-        if (t1 != 1 and width > 1) or t0 < width:
-            raise ValueError(f"table: rows must be packed and must not overlap, strides {table.stride()}")
-        lp = _ints("lens", lens, B, _I32, dev)
-        out, op = _output("out", out, B, hq, d, q, dev)
-        handle = _current(dev) if stream is None else _stream(stream, dev, (
-            q, table, lens, out, c.k, c.v, c.k_scale, c.v_scale, self._ws))
-        rc = self._fn(c._ref, qp, qs, B, hq, table.data_ptr(), width, t0, lp, self.scale, op, self._wsp, handle)
-        if rc:
-            _abi.check("colizig_cuda_attn_decode", rc)
-        return out
+        dev = c._index
+        if stream is None:
+            handle = _current(dev)
+        else:
+            handle, s = _elsewhere(stream, dev)
+            if s is not None:
+                _mark(s, q, table, lens, out, c.k, c.v, c.k_scale, c.v_scale, self._ws)
+                out = _room(s, out, q.shape, c.device)
+        r = c._lib.decode(c._at, dev, self.q_heads, self.max_batch, self.scale, self._wsp, q, table, lens, out, handle)
+        if r.__class__ is int:
+            _abi.check("colizig_cuda_attn_decode", r)
+        return r
 
 
 def prefill(q, k, v, cu_q, cu_k=None, scale: Optional[float] = None, out=None, stream=None):
@@ -266,30 +211,23 @@ def prefill(q, k, v, cu_q, cu_k=None, scale: Optional[float] = None, out=None, s
     strides free; cu i32 [B + 1], cu_k defaults to cu_q).  Queries are the last tokens of
     their sequence; a query that sees no key gives zeros; rows past the last sequence's are not written.  scale
     defaults to head_dim ** -0.5."""
-    dev, d = q.get_device(), q.shape[-1]
-    if dev < 0 or d not in HEAD_DIMS:
-        raise ValueError(f"q must be a CUDA tensor of head_dim {HEAD_DIMS}, got {tuple(q.shape)} on {q.device}")
+    dev = q.get_device()
+    if dev < 0:
+        raise ValueError(f"q must be a CUDA tensor, got one on {q.device}")
     _ready(dev)
-    Tq, hq, qs, qp = _rows("q", q, None, d, _BF16, dev)
-    Tk, hk, ks, kp = _rows("k", k, None, d, _BF16, dev)
-    tv, _, vs, vp = _rows("v", v, hk, d, _BF16, dev)
-    if hk < 1 or hq < 1 or hq % hk or tv != Tk:
-        raise ValueError(f"q {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)} do not belong together")
-    if cu_k is None:
-        cu_k = cu_q
-        if Tk != Tq:
-            raise ValueError("without cu_k, q and k must hold the same tokens")
-    n = cu_q.shape[0]
-    if n < 1:
-        raise ValueError("cu_q must hold at least the leading 0")
-    cq, ck = _ints("cu_q", cu_q, n, _I32, dev), _ints("cu_k", cu_k, n, _I32, dev)
-    out, op = _output("out", out, Tq, hq, d, q, dev)
-    handle = _current(dev) if stream is None else _stream(stream, dev, (q, k, v, cu_q, cu_k, out))
-    rc = _abi.load().colizig_cuda_attn_prefill(qp, kp, vp, qs, ks, vs, Tq, Tk, n - 1, hq, hk, d, cq, ck,
-                                               d ** -0.5 if scale is None else scale, op, handle)
-    if rc:
-        _abi.check("colizig_cuda_attn_prefill", rc)
-    return out
+    if scale is None:
+        scale = q.shape[-1] ** -0.5
+    if stream is None:
+        handle = _current(dev)
+    else:
+        handle, s = _elsewhere(stream, dev)
+        if s is not None:
+            _mark(s, q, k, v, cu_q, cu_k, out)
+            out = _room(s, out, q.shape, q.device)
+    r = _native().prefill(dev, q, k, v, cu_q, cu_k, scale, out, handle)
+    if r.__class__ is int:
+        _abi.check("colizig_cuda_attn_prefill", r)
+    return r
 
 
 def check(stream=None) -> None:
