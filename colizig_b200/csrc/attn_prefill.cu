@@ -14,8 +14,9 @@
 // tokens.  Keys and values are read once for all of them, a short prompt still fills
 // the tile (16 tokens of 8 heads), and the diagonal wastes at most 16 of 128 keys there.
 //
-// One block per SM runs through pairs of query tiles, the longest first and in turn from either
-// end, so that the blocks end together; the next pair's queries, keys and first products go out
+// One block per SM runs through pairs of query tiles (single ones where SMs would idle: 927 tokens of 8
+// heads on one, 21.7 -> 16.2 us), the longest first and in turn from either end, so that the blocks
+// end together; the next pair's queries, keys and first products go out
 // while the last one's results are written.  Warps: 0-3 and 4-7 softmax of query tile 0 and 1 (a
 // thread a row), 8 TMA loads, 9 MMA issue, 10 picks the pairs, 11 clears what lies behind the last
 // values.
@@ -48,7 +49,9 @@ struct PrefillArgs {
     CUtensorMap qmap, kmap, vmap;  // [rows][heads][D] in boxes of 64 columns
     AttnPrefillParams p;
     int group, pack, tokens;       // query heads per kv head; heads and tokens of a query tile
+    int step;                      // tokens of a block's turn: two query tiles', or one's (then the second is empty)
     int htiles;                    // passes over a group's heads
+    uint32_t sms;
 };
 
 template <int D>
@@ -227,7 +230,9 @@ __device__ __forceinline__ int reach(int nq, int nk, int step, int x) {
 struct Bounds {
     int q0, nq, k0, nk;
 };
-__device__ __forceinline__ Pair pick(const AttnPrefillParams& p, int step, int rank, const Bounds& own) {
+// Order is by the reach in multiples of this many keys: finer than a tile, and few halvings.
+constexpr int kGrain = 32;
+__device__ __forceinline__ Pair pick(const AttnPrefillParams& p, int step, int rank, const Bounds& own, bool sorted) {
     const int lane = threadIdx.x & 31;
     auto get = [&](int b, int& q0, int& nq, int& k0, int& nk) {
         if (b < 32) q0 = own.q0, nq = own.nq, k0 = own.k0, nk = own.nk;
@@ -239,7 +244,7 @@ __device__ __forceinline__ Pair pick(const AttnPrefillParams& p, int step, int r
         for (int b = lane; b < p.B; b += 32) {
             int q0, nq, k0, nk;
             get(b, q0, nq, k0, nk);
-            c += reach(nq, nk, step, x);
+            c += reach(nq, nk, step, x * kGrain);
         }
         return (int)__reduce_add_sync(0xffffffffu, (unsigned)c);
     };
@@ -249,28 +254,31 @@ __device__ __forceinline__ Pair pick(const AttnPrefillParams& p, int step, int r
         const int n = (nq + step - 1) / step;
         tile = rank < n ? n - 1 - rank : -1;
     } else {
-        int top = 0;  // past every reach
-#pragma unroll 1
-        for (int b = lane; b < p.B; b += 32) {
-            get(b, q0, nq, k0, nk);
-            top = max(top, nk + step);
-        }
-        top = (int)__reduce_max_sync(0xffffffffu, (unsigned)top) + 1;
         if (count(0) > rank) {
-            int lo = 0, hi = top;  // count(lo) > rank >= count(hi)
-            while (hi - lo > 1) {
-                const int mid = lo + (hi - lo) / 2;
-                if (count(mid) > rank) lo = mid;
-                else hi = mid;
+            int lo = 0, hi = 0x3fffffff / kGrain;  // count(lo) > rank >= count(hi); unsorted: all at once
+            if (sorted) {
+                int top = 0;  // past every reach
+#pragma unroll 1
+                for (int b = lane; b < p.B; b += 32) {
+                    get(b, q0, nq, k0, nk);
+                    top = max(top, nk + step);
+                }
+                hi = (int)__reduce_max_sync(0xffffffffu, (unsigned)top) / kGrain + 1;
+#pragma unroll 1
+                while (hi - lo > 1) {
+                    const int mid = lo + (hi - lo) / 2;
+                    if (count(mid) > rank) lo = mid;
+                    else hi = mid;
+                }
             }
-            int left = rank - count(hi);  // which of the pairs that reach lo but not hi
+            int left = sorted ? rank - count(hi) : rank;  // which of the pairs that reach lo but not hi
             for (int b0 = 0; b0 < p.B; b0 += 32) {
                 const int b = b0 + lane;
                 int c = 0;
                 q0 = nq = k0 = nk = 0;
                 if (b < p.B) {
                     get(b, q0, nq, k0, nk);
-                    c = reach(nq, nk, step, lo) - reach(nq, nk, step, hi);
+                    c = reach(nq, nk, step, lo * kGrain) - (sorted ? reach(nq, nk, step, hi * kGrain) : 0);
                 }
                 int inc = c;
 #pragma unroll
@@ -282,7 +290,7 @@ __device__ __forceinline__ Pair pick(const AttnPrefillParams& p, int step, int r
                 if (hit) {
                     const int src = __ffs(hit) - 1;
                     const int n = (nq + step - 1) / step;
-                    const int t = n - reach(nq, nk, step, lo) + (left - (inc - c));
+                    const int t = n - reach(nq, nk, step, lo * kGrain) + (left - (inc - c));
                     tile = __shfl_sync(0xffffffffu, t, src);
                     q0 = __shfl_sync(0xffffffffu, q0, src);
                     nq = __shfl_sync(0xffffffffu, nq, src);
@@ -305,9 +313,9 @@ struct Work {
     int last_keys;
     bool unclean;
 
-    __device__ __forceinline__ Work(const Pair& w, int tokens) {
-        tok0 = w.tile * 2 * tokens;
-        tok1 = tok0 + tokens;
+    __device__ __forceinline__ Work(const Pair& w, int tokens, int step) {
+        tok0 = w.tile * step;
+        tok1 = step > tokens ? tok0 + tokens : w.nq;
         const int a = min(w.nq, tok0 + tokens) - 1 + w.nk - w.nq, b = min(w.nq, tok1 + tokens) - 1 + w.nk - w.nq;
         n0 = tok0 >= w.nq || a < 0 ? 0 : a / kKeys + 1;
         n1 = tok1 >= w.nq || b < 0 ? 0 : b / kKeys + 1;
@@ -399,7 +407,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefill_kernel(const __grid_
             Pair w;
 #pragma unroll 1
             for (int t = 0; ok && next_pair(t, w); ++t) {
-                const Work k(w, A.tokens);
+                const Work k(w, A.tokens, A.step);
                 const int kh = w.head / A.htiles, head = kh * A.group + (w.head % A.htiles) * A.pack;
                 auto load_q = [&](int i) {
                     if (k.n(i) == 0) return true;
@@ -471,7 +479,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefill_kernel(const __grid_
             Pair w;
 #pragma unroll 1
             for (int t = 0; ok && next_pair(t, w); ++t) {
-                const Work work(w, A.tokens);
+                const Work work(w, A.tokens, A.step);
                 if (work.most == 0) continue;
                 ok = wait_kv();
                 int kst = next_kv();
@@ -540,6 +548,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefill_kernel(const __grid_
         } else if (warp == 10) {
             // ---------------- the block's pairs, in turn from either end of each round ----------------
             const int heads = (int)p.kv_heads * A.htiles;
+            const bool sorted = gridDim.x == A.sms;  // (fewer blocks: a turn each, in any order)
             Bounds own = {0, 0, 0, 0};
             if (lane < p.B && !bounds(p, lane, own.q0, own.nq, own.k0, own.nk)) atomicOr(p.err, kAttnErrIndex);
             if (blockIdx.x == 0) {
@@ -556,7 +565,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefill_kernel(const __grid_
                     break;
                 }
                 const uint32_t item = t * gridDim.x + (t & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
-                Pair w = pick(p, 2 * A.tokens, (int)(item / heads), own);
+                Pair w = pick(p, A.step, (int)(item / heads), own, sorted);
                 w.head = (int)(item % heads);
                 if (lane == 0) {
                     B.pairs[at] = w;
@@ -571,7 +580,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefill_kernel(const __grid_
             Pair w;
 #pragma unroll 1
             for (int t = 0; next_pair(t, w); ++t) {
-                const Work k(w, A.tokens);
+                const Work k(w, A.tokens, A.step);
                 uses += 2 * k.most;
                 if (!k.unclean) continue;
                 if (!__all_sync(0xffffffffu, wait_bar(&B.vask, phase, abort))) {
@@ -603,7 +612,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefill_kernel(const __grid_
         Pair w;
 #pragma unroll 1
         for (int turn = 0; ok && next_pair(turn, w); ++turn) {
-            const Work work(w, A.tokens);
+            const Work work(w, A.tokens, A.step);
             const int tok = i ? work.tok1 : work.tok0, tiles = work.n(i);
             const int kh = w.head / A.htiles, head0 = (w.head % A.htiles) * A.pack;  // first query head of the group's pass
             const int t = tok + lt;
@@ -773,9 +782,14 @@ int attn_prefill_launch(const AttnPrefillParams& p, int num_sms, cudaStream_t st
     a.htiles = (a.group + 127) / 128;
     a.pack = (a.group + a.htiles - 1) / a.htiles;
     a.tokens = 128 / a.pack;
-    const uint64_t pairs = ((uint64_t)p.Tq / (2 * a.tokens) + p.B) * p.kv_heads * a.htiles;  // at most
-    if (pairs > 0x3fffffffu) return CZ_ESHAPE;
-    const uint32_t grid = pairs < (uint64_t)num_sms ? (uint32_t)pairs : (uint32_t)num_sms;
+    // turns at most; one query tile each where that still leaves SMs idle
+    const uint64_t heads = (uint64_t)p.kv_heads * a.htiles;
+    const uint64_t single = ((uint64_t)p.Tq / a.tokens + p.B) * heads;
+    a.step = single <= (uint64_t)num_sms ? a.tokens : 2 * a.tokens;
+    const uint64_t turns = ((uint64_t)p.Tq / a.step + p.B) * heads;
+    if (turns > 0x3fffffffu) return CZ_ESHAPE;
+    a.sms = (uint32_t)num_sms;
+    const uint32_t grid = turns < (uint64_t)num_sms ? (uint32_t)turns : (uint32_t)num_sms;
     if (!make_map(&a.qmap, p.q, p.Tq, p.q_heads, p.head_dim, p.q_stride, a.pack, a.tokens) ||
         !make_map(&a.kmap, p.k, p.Tk, p.kv_heads, p.head_dim, p.k_stride, 1, kKeys) ||
         !make_map(&a.vmap, p.v, p.Tk, p.kv_heads, p.head_dim, p.v_stride, 1, kKeys))

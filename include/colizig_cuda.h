@@ -368,7 +368,7 @@ int colizig_cuda_attn_append(const colizig_kv_cache* cache, const void* q, const
  * head_dim] at q_stride elements a sequence, table int32 [B, table_width] at
  * table_stride, lens int32 [B]; out bf16 [B, q_heads, head_dim].  A sequence of length 0
  * gives zeros.  Rows of a page past the length may hold anything, NaN included.
- * B is at most COLIZIG_ATTN_MAX_BATCH.  workspace: colizig_cuda_attn_decode_workspace
+ * B is at most COLIZIG_ATTN_MAX_BATCH, and B * kv_heads * table_width * page_size / 16 under 2^31 (else -8).  workspace: colizig_cuda_attn_decode_workspace
  * bytes, 256-byte aligned and zeroed once before its first use; each call leaves it
  * ready for the next.  Calls that may overlap in time need a workspace each. */
 #define COLIZIG_ATTN_MAX_BATCH 4096

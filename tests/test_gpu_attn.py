@@ -176,6 +176,20 @@ def test_decode_many_ragged(hq, hk, d, page, e4m3):
     attn.check()
 
 
+@pytest.mark.parametrize("lens", [[61] * 28, [32] * 101, [7 * i % 119 for i in range(112)], [496] * 21, [1] * 148])
+@pytest.mark.parametrize("e4m3", [False, True])
+def test_decode_many_short(lens, e4m3):
+    """More short items than blocks: four, two or one warp each, none cut between blocks."""
+    g = gen(len(lens) + e4m3)
+    pg = Paged(g, lens, 8, 128, 32, e4m3)
+    q = randn(g, len(lens), 16, 128, dtype=torch.bfloat16) * 2
+    plan = attn.DecodePlan(pg.cache, 16, len(lens))
+    got = plan.run(q, pg.table, pg.len_t)
+    close(got, *pg.want(q, 128 ** -0.5))
+    assert torch.equal(plan.run(q, pg.table, pg.len_t), got)
+    attn.check()
+
+
 @pytest.mark.parametrize("hk,d,e4m3", [(1, 64, False), (1, 128, True), (2, 128, False)])
 def test_decode_one_item_over_all_blocks(hk, d, e4m3):
     """Few pairs on a long cache: partials of up to all blocks joined, groups of 8 and of 16 heads."""
