@@ -782,10 +782,16 @@ int attn_prefill_launch(const AttnPrefillParams& p, int num_sms, cudaStream_t st
     a.htiles = (a.group + 127) / 128;
     a.pack = (a.group + a.htiles - 1) / a.htiles;
     a.tokens = 128 / a.pack;
-    // turns at most; one query tile each where that still leaves SMs idle
+    // Turns at most. One query tile each where that still leaves SMs idle, and for one long prompt
+    // whose pairs would: the last pair, which is the longest, then bounds the call. Measured for
+    // one prompt, single tiles against pairs: 8 heads on 1, 2,400 tokens 32.1 against 35.8 us, 4,600
+    // 58.2 against 63.2; 12 on 2, 2,500 tokens 37.1 against 40.1; but 32 on 4, 1,100 tokens 23.1
+    // against 22.0, and 4 prompts of 900 tokens in all (which then need the sort) 18.1 against 12.2.
     const uint64_t heads = (uint64_t)p.kv_heads * a.htiles;
     const uint64_t single = ((uint64_t)p.Tq / a.tokens + p.B) * heads;
-    a.step = single <= (uint64_t)num_sms ? a.tokens : 2 * a.tokens;
+    const uint64_t pairs = ((uint64_t)p.Tq / (2 * a.tokens) + p.B) * heads;
+    const bool lone = p.B == 1 && p.Tk >= 2048 && pairs <= (uint64_t)num_sms;
+    a.step = single <= (uint64_t)num_sms || lone ? a.tokens : 2 * a.tokens;
     const uint64_t turns = ((uint64_t)p.Tq / a.step + p.B) * heads;
     if (turns > 0x3fffffffu) return CZ_ESHAPE;
     a.sms = (uint32_t)num_sms;
