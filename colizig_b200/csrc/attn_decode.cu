@@ -54,7 +54,7 @@ constexpr int kBatch = 40;         // partials of other blocks joined at a time
 constexpr int kSlotFloats = kMaxTiles * 8 * 128 + kMaxTiles * 8 * 2;  // o, then (m, l) per head
 
 struct DecodeArgs {
-    CUtensorMap kmap, vmap;  // [pages][kv_heads][page_size][head_dim], boxes of 16 rows x up to 128 bytes
+    CUtensorMap kmap, vmap;  // page, head, column block, row, columns of the block (128 bytes at most)
     AttnDecodeParams p;
     uint32_t group, tiles;   // query heads per kv head; passes of NT * 8 of them
     float* slots;            // workspace: [grid][2][kSlotFloats]
