@@ -1145,8 +1145,9 @@ CZ_EXPORT int colizig_cuda_moe_register_layer(uint32_t layer, const colizig_moe_
     L.e_hi = e_hi;
     L.shared_here = shared_here;
     L.ep = ep;
-    if (cudaMalloc(&L.mem, off) != cudaSuccess) return CZ_EALLOC;
-    uint8_t* base = reinterpret_cast<uint8_t*>(L.mem);
+    // cudaMalloc gives small blocks on 512 bytes when others came before them: the layer's start is rounded up here
+    if (cudaMalloc(&L.mem, off + 1023) != cudaSuccess) return CZ_EALLOC;
+    uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(L.mem) + 1023) & ~uintptr_t(1023));
     L.router = reinterpret_cast<float*>(base + o_router);
     L.gate_w = base + o_gw;
     L.up_w = base + o_uw;
