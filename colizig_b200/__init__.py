@@ -15,13 +15,19 @@ the reference's host-side interfaces:
   checkpoint  src/model/weights.zig + moe.zig Layer.load / loadExpert: one MoE
         layer from safetensors shards straight into resident device memory
   attn  the attention between the FP8 projections: rotation and paged cache
-        write, attention of one new token, attention over whole prompts
+        write, attention of one new token, attention over whole prompts (torch
+        tensors only: absent where torch is)
 
 There is no CPU fallback: if the library is missing or a call fails, an
 exception is raised.
 """
 
-from . import _abi, attn, checkpoint, ep, fp8, gpu, moe  # noqa: F401
+from . import _abi, checkpoint, ep, fp8, gpu, moe  # noqa: F401
 from ._abi import ColizigError  # noqa: F401
 
-__all__ = ["gpu", "fp8", "moe", "ep", "checkpoint", "attn", "ColizigError"]
+__all__ = ["gpu", "fp8", "moe", "ep", "checkpoint", "ColizigError"]
+
+if moe.torch is not None:
+    from . import attn  # noqa: F401
+
+    __all__.append("attn")
