@@ -120,6 +120,16 @@ double real(PyObject* o) {
 }
 std::string number(int64_t v) { return std::to_string(v); }
 
+// The library's calls run without the interpreter lock: they wait for the library's mutex, which another thread's
+// host-pointer call holds until its stream has finished.
+template <class F>
+int unlocked(F call) {
+    PyThreadState* state = PyEval_SaveThread();
+    const int rc = call();
+    PyEval_RestoreThread(state);
+    return rc;
+}
+
 template <class F>
 PyObject* guarded(Py_ssize_t n, Py_ssize_t want, F body) {
     if (n != want) {
@@ -187,11 +197,14 @@ PyObject* append(PyObject*, PyObject* const* a, Py_ssize_t n) {
         void* qp = output("q_out", a[12], q.n, q.heads, d, tq, index, qo);
         void* kp = packed || a[13] != Py_None ? output("k_out", a[13], q.n, hk, d, tk, index, ko) : nullptr;
         void* vp = packed || a[14] != Py_None ? output("v_out", a[14], q.n, hk, d, tk, index, vo) : nullptr;
-        const int rc = lib_append(cache, q.at, k.at, v.at, dt == at::kFloat ? COLIZIG_X_F32 : COLIZIG_X_BF16, (int)q.n,
-                                  (uint32_t)q.heads, q.stride, k.stride, v.stride, static_cast<const int32_t*>(positions),
-                                  static_cast<const int64_t*>(slots), static_cast<const float*>(rope), (uint32_t)rope_len,
-                                  (uint32_t)rot, static_cast<const float*>(qn), static_cast<const float*>(kn), eps, qp, kp,
-                                  vp, address(a[15]));
+        void* stream = address(a[15]);
+        const int rc = unlocked([&] {
+            return lib_append(cache, q.at, k.at, v.at, dt == at::kFloat ? COLIZIG_X_F32 : COLIZIG_X_BF16, (int)q.n,
+                              (uint32_t)q.heads, q.stride, k.stride, v.stride, static_cast<const int32_t*>(positions),
+                              static_cast<const int64_t*>(slots), static_cast<const float*>(rope), (uint32_t)rope_len,
+                              (uint32_t)rot, static_cast<const float*>(qn), static_cast<const float*>(kn), eps, qp, kp, vp,
+                              stream);
+        });
         if (rc) return PyLong_FromLong(rc);
         PyObject* out[3] = {wrapped(a[12], qo), wrapped(a[13], ko), wrapped(a[14], vo)};
         PyObject* t = out[0] && out[1] && out[2] ? PyTuple_Pack(3, out[0], out[1], out[2]) : nullptr;
@@ -217,10 +230,14 @@ PyObject* decode(PyObject*, PyObject* const* a, Py_ssize_t n) {
         const void* lens = vector("lens", tensor("lens", a[8]), q.n, at::kInt, index, false);
         at::Tensor o;
         void* op = output("out", a[9], q.n, hq, d, tq, index, o);
-        const int rc = lib_decode(cache, q.at, q.stride, (int)q.n, (uint32_t)hq,
-                                  static_cast<const int32_t*>(t.const_data_ptr()), (uint32_t)t.size(1),
-                                  q.n > 1 ? t.stride(0) : t.size(1), static_cast<const int32_t*>(lens), (float)real(a[4]), op,
-                                  address(a[5]), address(a[10]));
+        const void* table = t.const_data_ptr();
+        const int64_t width = t.size(1), row = q.n > 1 ? t.stride(0) : width;
+        const float scale = (float)real(a[4]);
+        void *workspace = address(a[5]), *stream = address(a[10]);
+        const int rc = unlocked([&] {
+            return lib_decode(cache, q.at, q.stride, (int)q.n, (uint32_t)hq, static_cast<const int32_t*>(table),
+                              (uint32_t)width, row, static_cast<const int32_t*>(lens), scale, op, workspace, stream);
+        });
         return rc ? PyLong_FromLong(rc) : wrapped(a[9], o);
     });
 }
@@ -248,9 +265,13 @@ PyObject* prefill(PyObject*, PyObject* const* a, Py_ssize_t n) {
         const void* ckp = same ? cqp : vector("cu_k", tensor("cu_k", a[5]), m, at::kInt, index, false);
         at::Tensor o;
         void* op = output("out", a[7], q.n, q.heads, d, tq, index, o);
-        const int rc = lib_prefill(q.at, k.at, v.at, q.stride, k.stride, v.stride, (int)q.n, (int)k.n, (int)(m - 1),
-                                   (uint32_t)q.heads, (uint32_t)k.heads, (uint32_t)d, static_cast<const int32_t*>(cqp),
-                                   static_cast<const int32_t*>(ckp), (float)real(a[6]), op, address(a[8]));
+        const float scale = (float)real(a[6]);
+        void* stream = address(a[8]);
+        const int rc = unlocked([&] {
+            return lib_prefill(q.at, k.at, v.at, q.stride, k.stride, v.stride, (int)q.n, (int)k.n, (int)(m - 1),
+                               (uint32_t)q.heads, (uint32_t)k.heads, (uint32_t)d, static_cast<const int32_t*>(cqp),
+                               static_cast<const int32_t*>(ckp), scale, op, stream);
+        });
         return rc ? PyLong_FromLong(rc) : wrapped(a[7], o);
     });
 }
