@@ -153,6 +153,7 @@ def append(cache: KvCache, q, k, v, positions, slots, rope=None, q_norm=None, k_
     page_size + row, negative: not cached, no slot twice), positions i32 [T].  Returns (q, k, v)
     packed in bf16; k and v (what ``prefill`` reads) are None unless packed or given."""
     dev = cache._index
+    _ready(dev)
     if stream is None:
         handle = _current(dev)
     else:
@@ -192,6 +193,7 @@ class DecodePlan:
         first tokens of the pages table[b] (i32 [B, width], row stride free; lens i32 [B])."""
         c = self.cache
         dev = c._index
+        _ready(dev)
         if stream is None:
             handle = _current(dev)
         else:

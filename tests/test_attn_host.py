@@ -1,6 +1,7 @@
 """Host side of the attention calls, without a GPU: tensors that only claim to lie on one, and stand-ins for the
 library's entry points."""
 
+import contextlib
 import ctypes
 import shutil
 import subprocess
@@ -11,7 +12,7 @@ import pytest
 
 torch = pytest.importorskip("torch")
 
-from colizig_b200 import _abi, attn  # noqa: E402
+from colizig_b200 import _abi, attn, gpu  # noqa: E402
 
 
 class OnPaper(torch.Tensor):
@@ -72,3 +73,47 @@ def test_other_threads_run_while_a_call_waits(native, tmp_path, which):
     ctypes.c_int.in_dll(L, "go").value = 1
     t.join(20)
     assert got == [41]  # 42: nobody could let it go
+
+
+@pytest.fixture
+def on_paper(native, monkeypatch):
+    """The library as if it were up on device 0, with entry points that count their calls and launch nothing, and a cache
+    and a plan of tensors without memory."""
+    done = []
+    at = ctypes.CFUNCTYPE(ctypes.c_int)(lambda: done.append(1) or 0)
+    native.bind(*[ctypes.cast(at, ctypes.c_void_p).value] * 3)
+    monkeypatch.setattr(gpu, "_ready", True)
+    monkeypatch.setattr(gpu, "_device", 0)
+    monkeypatch.setattr(attn, "_current", lambda index: 0)
+    cache = attn.KvCache(paper(2, 2, 16, 128), paper(2, 2, 16, 128))
+    with monkeypatch.context() as m:
+        m.setattr(torch, "zeros", lambda *a, **k: paper(1024, dtype=torch.uint8))
+        m.setattr(torch.cuda, "device", lambda d: contextlib.nullcontext())
+        plan = attn.DecodePlan(cache, 4, 2)
+    yield cache, plan, done
+    del at
+
+
+def python_calls(cache, plan):
+    q, kv, i32 = paper(2, 4, 128), paper(2, 2, 128), paper(2, dtype=torch.int32)
+    return [lambda: attn.append(cache, q, kv, kv, None, paper(2, dtype=torch.int64), q_out=paper(2, 4, 128)),
+            lambda: plan.run(q, paper(2, 3, dtype=torch.int32), i32, out=paper(2, 4, 128)),
+            lambda: attn.prefill(q, kv, kv, i32, out=paper(2, 4, 128))]
+
+
+def test_calls_go_through_on_the_library_s_device(on_paper):
+    cache, plan, done = on_paper
+    for f in python_calls(cache, plan):
+        f()
+    assert len(done) == 3
+
+
+def test_calls_are_refused_when_the_library_moved_to_another_device(on_paper, monkeypatch):
+    """A cache and a plan made before a shutdown and an init on another device: the kernels would run there, on the first
+    device's addresses."""
+    cache, plan, done = on_paper
+    monkeypatch.setattr(gpu, "_device", 1)
+    for f in python_calls(cache, plan):
+        with pytest.raises(ValueError, match="cuda:0, the library runs on cuda:1"):
+            f()
+    assert not done
