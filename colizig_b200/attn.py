@@ -234,6 +234,7 @@ def prefill(q, k, v, cu_q, cu_k=None, scale: Optional[float] = None, out=None, s
 
 def check(stream=None) -> None:
     """Raise if an attention call since the last check met an index outside its buffer (slot,
-    position, page, length or sequence bound).  Waits for `stream` (default: the current one)."""
-    handle = _current(torch.cuda.current_device()) if stream is None else getattr(stream, "cuda_stream", stream)
+    position, page, length or sequence bound).  Waits for `stream` (default: the current one of the library's
+    device)."""
+    handle = _current(gpu.device()) if stream is None else getattr(stream, "cuda_stream", stream)
     _abi.check("colizig_cuda_attn_check", _abi.load().colizig_cuda_attn_check(handle))

@@ -117,3 +117,22 @@ def test_calls_are_refused_when_the_library_moved_to_another_device(on_paper, mo
         with pytest.raises(ValueError, match="cuda:0, the library runs on cuda:1"):
             f()
     assert not done
+
+
+def test_check_waits_for_a_stream_of_the_library_s_device(monkeypatch):
+    """Not of torch's current device, whose stream the library's device cannot wait for."""
+    seen = []
+
+    class Library:
+        @staticmethod
+        def colizig_cuda_attn_check(handle):
+            seen.append(handle)
+            return 0
+
+    monkeypatch.setattr(gpu, "_device", 3)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    monkeypatch.setattr(attn, "_current", lambda index: 1000 + index)
+    monkeypatch.setattr(_abi, "load", lambda: Library)
+    attn.check()
+    attn.check(stream=7)
+    assert seen == [1003, 7]
