@@ -188,7 +188,7 @@ struct Ctx {
     HostBuf mm_xh, mm_yh;  // pinned staging of colizig_cuda_matmul_fp8's x and y (up to kHostStageCap bytes)
     HostBuf io_xh;    // pinned staging of the tokens (host-pointer forward, up to kHostStageCap bytes)
     uint32_t* sync = nullptr;
-    uint32_t* attn_err = nullptr;  // the attention calls' error word
+    uint32_t* attn_err = nullptr;  // the attention calls' error word (attn_error_word's address)
     // expert parallelism (one process per GPU)
     bool ep_on = false;
     int ep_rank = 0, ep_world = 1;
@@ -265,6 +265,10 @@ NcclApi nccl;
 
 Ctx g;
 std::mutex g_mu;
+
+// The attention calls' error word.  Not from the allocator: graphs captured by the caller hold its address, also
+// after a shutdown.
+__device__ uint32_t attn_error_word;
 
 // A host wait with a deadline.  query(): 0 done, 1 pending, < 0 failed;
 // async_error(): true when the communicator reports an error of its own;
@@ -489,7 +493,6 @@ void shutdown_locked() {
                       &g.sh_tmp, &g.sh_send, &g.sh_recv, &g.sh_x, &g.sh_ridx, &g.sh_rgates, &g.sh_part, &g.sh_back})
         b->release();
     if (g.sync) cudaFree(g.sync);
-    if (g.attn_err) cudaFree(g.attn_err);
     for (cudaEvent_t e : g.tm_ev) cudaEventDestroy(e);
     if (g.stream) cudaStreamDestroy(g.stream);
     g = Ctx{};
@@ -509,15 +512,15 @@ int init_locked(int device) {
     g.num_sms = prop.multiProcessorCount;
     g.dev = device;
     if (cudaStreamCreateWithFlags(&g.stream, cudaStreamNonBlocking) != cudaSuccess) return -4;
-    // allocated here, not on first use: an attention call may be inside a stream capture
-    if (cudaMalloc(&g.attn_err, sizeof(uint32_t)) != cudaSuccess ||
-        cudaMemset(g.attn_err, 0, sizeof(uint32_t)) != cudaSuccess || cudaStreamSynchronize(nullptr) != cudaSuccess) {
-        if (g.attn_err) cudaFree(g.attn_err);
-        g.attn_err = nullptr;
+    // looked up here, not on first use: an attention call may be inside a stream capture
+    void* word = nullptr;
+    if (cudaGetSymbolAddress(&word, attn_error_word) != cudaSuccess ||
+        cudaMemset(word, 0, sizeof attn_error_word) != cudaSuccess || cudaStreamSynchronize(nullptr) != cudaSuccess) {
         cudaStreamDestroy(g.stream);
         g.stream = nullptr;
         return -4;
     }
+    g.attn_err = static_cast<uint32_t*>(word);
     g.budget = 0;  // keyed store disabled until set (colizig_cuda.cu:184)
     g.inited = true;
     ++cz::init_serial;

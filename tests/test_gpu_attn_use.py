@@ -1,0 +1,44 @@
+"""Attention calls as a longer-lived program makes them: graphs kept over a shutdown, other streams, error words,
+buffers in odd states.  (Results against the definitions: test_gpu_attn.py, whose helpers are used here.)"""
+
+import pytest
+
+torch = pytest.importorskip("torch")
+
+from colizig_b200 import ColizigError, attn, gpu  # noqa: E402
+from tests.test_gpu_attn import Paged, close, gen, prefill_want, prompts, randn  # noqa: E402,F401
+
+pytestmark = pytest.mark.gpu
+
+
+def reported():
+    """The error word as a check reports it: its code, or 0."""
+    try:
+        attn.check()
+    except ColizigError as e:
+        return e.rc
+    return 0
+
+
+def test_graph_kept_over_a_shutdown_reports_to_the_new_library():
+    """A captured call holds the error word's address: it stays good after a shutdown and another init."""
+    g = gen(70)
+    pg = Paged(g, [100, 40], 2, 64, 16)
+    q = randn(g, 2, 4, 64, dtype=torch.bfloat16)
+    plan = attn.DecodePlan(pg.cache, 4, 2)
+    lens = pg.len_t.clone()
+    want = plan.run(q, pg.table, lens)
+    out = torch.empty_like(want)
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        plan.run(q, pg.table, lens, out=out)
+    gpu.deinit()
+    gpu.init()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, want) and reported() == 0
+    lens[1] = -1
+    graph.replay()
+    torch.cuda.synchronize()
+    assert reported() == -11 and reported() == 0
