@@ -266,9 +266,12 @@ NcclApi nccl;
 Ctx g;
 std::mutex g_mu;
 
-// The attention calls' error word.  Not from the allocator: graphs captured by the caller hold its address, also
-// after a shutdown.
-__device__ uint32_t attn_error_word;
+// The attention calls' error word, and its value as the last check took it.  Not from the allocator: graphs captured by
+// the caller hold its address, also after a shutdown.
+__device__ uint32_t attn_error_word[2];
+
+// Reads and clears in one step: what a call on another stream reports after it stays for the next check.
+__global__ void attn_take_error(uint32_t* word) { word[1] = atomicExch(word, 0u); }
 
 // A host wait with a deadline.  query(): 0 done, 1 pending, < 0 failed;
 // async_error(): true when the communicator reports an error of its own;
@@ -1967,11 +1970,11 @@ CZ_EXPORT int colizig_cuda_attn_check(void* stream) {
     if (!g.inited) return CZ_EARGS;
     cudaSetDevice(g.dev);
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+    void* args[] = {&g.attn_err};
+    if (cudaLaunchKernel(attn_take_error, dim3(1), dim3(1), args, 0, st) != cudaSuccess) return CZ_ELAUNCH;
     uint32_t err = 0;
-    if (cudaMemcpyAsync(&err, g.attn_err, sizeof err, cudaMemcpyDeviceToHost, st) != cudaSuccess) return CZ_ED2H;
+    if (cudaMemcpyAsync(&err, g.attn_err + 1, sizeof err, cudaMemcpyDeviceToHost, st) != cudaSuccess) return CZ_ED2H;
     if (const int rc = stream_sync(st)) return rc;
     if (!err) return CZ_OK;
-    if (cudaMemsetAsync(g.attn_err, 0, sizeof err, st) != cudaSuccess) return CZ_ELAUNCH;
-    if (const int rc = stream_sync(st)) return rc;
     return err & cz::kAttnErrWait ? CZ_ETIMEOUT : CZ_EINDEX;
 }

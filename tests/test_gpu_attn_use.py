@@ -1,6 +1,9 @@
 """Attention calls as a longer-lived program makes them: graphs kept over a shutdown, other streams, error words,
 buffers in odd states.  (Results against the definitions: test_gpu_attn.py, whose helpers are used here.)"""
 
+import threading
+import time
+
 import pytest
 
 torch = pytest.importorskip("torch")
@@ -41,4 +44,43 @@ def test_graph_kept_over_a_shutdown_reports_to_the_new_library():
     lens[1] = -1
     graph.replay()
     torch.cuda.synchronize()
+    assert reported() == -11 and reported() == 0
+
+
+def test_errors_after_a_check_s_read_are_kept_for_the_next():
+    """A check queued behind a long kernel, a graph that meets a bad length queued behind the check's read while the
+    check still waits: the first check reports what was there, the second the graph's."""
+    g = gen(71)
+    pg = Paged(g, [100, 40], 2, 64, 16)
+    q = randn(g, 2, 4, 64, dtype=torch.bfloat16)
+    plan = attn.DecodePlan(pg.cache, 4, 2)
+    bad = pg.len_t.clone()
+    bad[0] = -5
+    plan.run(q, pg.table, bad)
+    out = torch.empty_like(q)
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        plan.run(q, pg.table, bad, out=out)
+    s = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    first = []
+
+    def check():
+        try:
+            attn.check(stream=s)
+            first.append(0)
+        except ColizigError as e:
+            first.append(e.rc)
+
+    with torch.cuda.stream(s):
+        torch.cuda._sleep(2_000_000_000)  # about a second
+    t = threading.Thread(target=check)
+    t.start()
+    time.sleep(0.3)
+    with torch.cuda.stream(s):
+        graph.replay()
+    t.join()
+    s.synchronize()
+    assert first == [-11]
     assert reported() == -11 and reported() == 0
