@@ -175,7 +175,7 @@ class DecodePlan:
     """Attention of one new token per sequence over `cache`, for up to max_batch sequences of
     q_heads query heads; scale defaults to head_dim ** -0.5.  Holds the workspace of the split
     over the cache's length, so calls of one plan must not overlap in time (one plan per
-    stream)."""
+    stream).  Making a plan waits for the current stream."""
 
     def __init__(self, cache: KvCache, q_heads: int, max_batch: int, scale: Optional[float] = None):
         _need(q_heads >= 1 and q_heads % cache.kv_heads == 0,
@@ -186,6 +186,9 @@ class DecodePlan:
         with torch.cuda.device(cache.device):
             self._ws = torch.zeros(_abi.load().colizig_cuda_attn_decode_workspace(), dtype=torch.uint8,
                                    device=cache.device)
+            # the zeros have landed before a call on any stream starts counting in them
+            if not torch.cuda.is_current_stream_capturing():
+                torch.cuda.current_stream().synchronize()
         self._wsp = self._ws.data_ptr()
 
     def run(self, q, table, lens, out=None, stream=None):

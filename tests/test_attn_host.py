@@ -89,6 +89,7 @@ def on_paper(native, monkeypatch):
     with monkeypatch.context() as m:
         m.setattr(torch, "zeros", lambda *a, **k: paper(1024, dtype=torch.uint8))
         m.setattr(torch.cuda, "device", lambda d: contextlib.nullcontext())
+        m.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
         plan = attn.DecodePlan(cache, 4, 2)
     yield cache, plan, done
     del at

@@ -84,3 +84,33 @@ def test_errors_after_a_check_s_read_are_kept_for_the_next():
     s.synchronize()
     assert first == [-11]
     assert reported() == -11 and reported() == 0
+
+
+def long_one(g, n=20000, hq=16, hk=2, d=128):
+    """A sequence cut between blocks, its queries and the right answer."""
+    pg = Paged(g, [n], hk, d, 64)
+    q = randn(g, 1, hq, d, dtype=torch.bfloat16)
+    want = attn.DecodePlan(pg.cache, hq, 1).run(q, pg.table, pg.len_t)
+    torch.cuda.synchronize()
+    return pg, q, want
+
+
+def test_a_new_plan_runs_on_another_stream_at_once():
+    """The workspace's zeros are queued on the stream where the plan is made, here behind a long kernel and over
+    memory that held something else: a first call on another stream must find them."""
+    pg, q, want = long_one(gen(72))
+    size = attn.DecodePlan(pg.cache, 16, 1)._ws.numel()
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    dirty = torch.full((size,), 255, dtype=torch.uint8, device="cuda")
+    s = torch.cuda.Stream()
+    out = torch.zeros_like(want)
+    torch.cuda.synchronize()
+    del dirty  # the plan's workspace takes its place
+    torch.cuda._sleep(400_000_000)
+    plan = attn.DecodePlan(pg.cache, 16, 1)
+    got = plan.run(q, pg.table, pg.len_t, out=out, stream=s)
+    s.synchronize()
+    assert torch.equal(got, want)
+    torch.cuda.synchronize()
+    assert torch.equal(plan.run(q, pg.table, pg.len_t), want)
