@@ -189,7 +189,7 @@ class DecodePlan:
             # the zeros have landed before a call on any stream starts counting in them
             if not torch.cuda.is_current_stream_capturing():
                 torch.cuda.current_stream().synchronize()
-        self._wsp = self._ws.data_ptr()
+        self._wsp, self._home = self._ws.data_ptr(), _current(cache._index)
 
     def run(self, q, table, lens, out=None, stream=None):
         """out [B, q_heads, head_dim] bf16 = attention of q (bf16, row stride free) over the lens[b]
@@ -197,13 +197,12 @@ class DecodePlan:
         c = self.cache
         dev = c._index
         _ready(dev)
-        if stream is None:
-            handle = _current(dev)
-        else:
-            handle, s = _elsewhere(stream, dev)
-            if s is not None:
-                _mark(s, q, table, lens, out, c.k, c.v, c.k_scale, c.v_scale, self._ws)
-                out = _room(s, out, q.shape, c.device)
+        handle, s = (_current(dev), None) if stream is None else _elsewhere(stream, dev)
+        if s is not None:
+            _mark(s, q, table, lens, out, c.k, c.v, c.k_scale, c.v_scale, self._ws)
+            out = _room(s, out, q.shape, c.device)
+        elif handle != self._home:  # the plan may be dropped while the call runs
+            self._ws.record_stream(torch.cuda.current_stream(dev))
         r = c._lib.decode(c._at, dev, self.q_heads, self.max_batch, self.scale, self._wsp, q, table, lens, out, handle)
         if r.__class__ is int:
             _abi.check("colizig_cuda_attn_decode", r)

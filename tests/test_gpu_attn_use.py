@@ -114,3 +114,22 @@ def test_a_new_plan_runs_on_another_stream_at_once():
     assert torch.equal(got, want)
     torch.cuda.synchronize()
     assert torch.equal(plan.run(q, pg.table, pg.len_t), want)
+
+
+def test_a_plan_dropped_while_its_call_waits_on_another_current_stream():
+    """The workspace is the plan's own: its memory is not handed out before the call on a stream that was made current
+    has run."""
+    pg, q, want = long_one(gen(73))
+    plan = attn.DecodePlan(pg.cache, 16, 1)
+    out = torch.zeros_like(want)
+    s = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(s):
+        torch.cuda._sleep(400_000_000)
+        plan.run(q, pg.table, pg.len_t, out=out)
+    size = plan._ws.numel()
+    del plan
+    other = [torch.full((size,), 255, dtype=torch.uint8, device="cuda") for _ in range(2)]
+    torch.cuda.synchronize()
+    assert torch.equal(out, want)
+    del other
