@@ -773,9 +773,6 @@ int launch(const PrefillArgs& a, uint32_t grid, cudaStream_t st) {
 }  // namespace
 
 int attn_prefill_launch(const AttnPrefillParams& p, int num_sms, cudaStream_t st) {
-    if (p.Tk == 0)  // no query sees a key
-        return cudaMemsetAsync(p.out, 0, (size_t)p.Tq * p.q_heads * p.head_dim * 2, st) == cudaSuccess ? CZ_OK
-                                                                                                      : CZ_ELAUNCH;
     PrefillArgs a{};
     a.p = p;
     a.group = (int)(p.q_heads / p.kv_heads);
@@ -796,10 +793,13 @@ int attn_prefill_launch(const AttnPrefillParams& p, int num_sms, cudaStream_t st
     if (turns > 0x3fffffffu) return CZ_ESHAPE;
     a.sms = (uint32_t)num_sms;
     const uint32_t grid = turns < (uint64_t)num_sms ? (uint32_t)turns : (uint32_t)num_sms;
-    if (!make_map(&a.qmap, p.q, p.Tq, p.q_heads, p.head_dim, p.q_stride, a.pack, a.tokens) ||
-        !make_map(&a.kmap, p.k, p.Tk, p.kv_heads, p.head_dim, p.k_stride, 1, kKeys) ||
-        !make_map(&a.vmap, p.v, p.Tk, p.kv_heads, p.head_dim, p.v_stride, 1, kKeys))
+    if (!make_map(&a.qmap, p.q, p.Tq, p.q_heads, p.head_dim, p.q_stride, a.pack, a.tokens)) return CZ_ESHAPE;
+    if (p.Tk == 0) {  // nothing is loaded then: the kernel checks the bounds and writes the sequences' zeros
+        a.kmap = a.vmap = a.qmap;
+    } else if (!make_map(&a.kmap, p.k, p.Tk, p.kv_heads, p.head_dim, p.k_stride, 1, kKeys) ||
+               !make_map(&a.vmap, p.v, p.Tk, p.kv_heads, p.head_dim, p.v_stride, 1, kKeys)) {
         return CZ_ESHAPE;
+    }
     return p.head_dim == 128 ? launch<128>(a, grid, st) : launch<64>(a, grid, st);
 }
 

@@ -133,3 +133,23 @@ def test_a_plan_dropped_while_its_call_waits_on_another_current_stream():
     torch.cuda.synchronize()
     assert torch.equal(out, want)
     del other
+
+
+@pytest.mark.parametrize("hq,hk,d", [(8, 2, 128), (3, 3, 64)])
+@pytest.mark.parametrize("nq", [[4, 0, 300], [1], [30] * 40])
+def test_prompts_on_no_keys_at_all(hq, hk, d, nq):
+    """Zeros for every query of a sequence; rows past the last sequence's are not written, bad bounds are reported."""
+    n = sum(nq)
+    q = randn(gen(74), n + 5, hq, d, dtype=torch.bfloat16)
+    kv = torch.empty((0, hk, d), device="cuda", dtype=torch.bfloat16)
+    cu = torch.tensor([0] + nq).cumsum(0).int().cuda()
+    none = torch.zeros_like(cu)
+    out = torch.full_like(q, 7.0)
+    attn.prefill(q, kv, kv, cu, none, out=out)
+    assert not out[:n].any() and (out[n:] == 7).all()
+    assert reported() == 0
+    for bad in ((cu, none.clone().index_fill_(0, torch.tensor([len(nq)], device="cuda"), 3)),
+                (cu.clone().index_fill_(0, torch.tensor([len(nq)], device="cuda"), n + 6), none)):
+        attn.prefill(q, kv, kv, *bad, out=out)
+        assert reported() == -11
+    assert (out[n:] == 7).all()
