@@ -254,6 +254,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) attn_decode_kernel(const __gri
         prefetch_tensormap(&A.vmap);
     }
 
+    __syncthreads();  // the flags are cleared before any warp's wait reads them
     pdl_wait();
 
     // ---- the line and this warp's part of it ----

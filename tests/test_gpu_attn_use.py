@@ -153,3 +153,16 @@ def test_prompts_on_no_keys_at_all(hq, hk, d, nq):
         attn.prefill(q, kv, kv, *bad, out=out)
         assert reported() == -11
     assert (out[n:] == 7).all()
+
+
+def test_decode_after_kernels_that_fill_shared_memory():
+    """A block's flags start cleared whatever the kernel before left in shared memory (here rotated keys and products of
+    all bits): no wait gives up early, results repeat."""
+    g = gen(75)
+    pg, q, want = long_one(g)
+    plan = attn.DecodePlan(pg.cache, 16, 1)
+    x, k, v, cu = prompts(g, [3000], [3000], 8, 2, 128, False)
+    for _ in range(100):
+        attn.prefill(x, k, v, cu[0])
+        assert torch.equal(plan.run(q, pg.table, pg.len_t), want)
+    assert reported() == 0
