@@ -37,19 +37,19 @@ template <int XBF16>
 __device__ __forceinline__ void load4(const void* base, uint64_t at, float* f) {
     if (XBF16) {
         uint2 r;
-        asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0, %1}, [%2];"
+        asm volatile("ld.global.L1::no_allocate.v2.u32 {%0, %1}, [%2];"
                      : "=r"(r.x), "=r"(r.y)
                      : "l"(reinterpret_cast<const uint16_t*>(base) + at));
         f[0] = __uint_as_float(r.x << 16), f[1] = __uint_as_float(r.x & 0xffff0000u);
         f[2] = __uint_as_float(r.y << 16), f[3] = __uint_as_float(r.y & 0xffff0000u);
     } else {
-        asm volatile("ld.global.nc.L1::no_allocate.v4.f32 {%0, %1, %2, %3}, [%4];"
+        asm volatile("ld.global.L1::no_allocate.v4.f32 {%0, %1, %2, %3}, [%4];"
                      : "=f"(f[0]), "=f"(f[1]), "=f"(f[2]), "=f"(f[3])
                      : "l"(reinterpret_cast<const float*>(base) + at));
     }
 }
 
-__device__ __forceinline__ float4 ldg4(const float* p) { return __ldg(reinterpret_cast<const float4*>(p)); }
+__device__ __forceinline__ float4 ldg4(const float* p) { return ld_now(reinterpret_cast<const float4*>(p)); }
 
 __device__ __forceinline__ uint2 pack_bf16x4(const float* f) {
     const __nv_bfloat162 a = __floats2bfloat162_rn(f[0], f[1]), b = __floats2bfloat162_rn(f[2], f[3]);
@@ -85,8 +85,8 @@ __global__ void __launch_bounds__(kThreads, HEADS == 4 ? 8 : 10) attn_append_ker
     const int e0 = turned ? 4 * sub : rot + 4 * (sub - turning);
     const int e1 = e0 + (turned ? rot : D - rot) / 2;
 
-    int pos = turned && live ? __ldg(p.positions + t) : 0;
-    const int64_t slot = live ? __ldg(p.slots + t) : -1;
+    int pos = turned && live ? ld_now(p.positions + t) : 0;
+    const int64_t slot = live ? ld_now(p.slots + t) : -1;
     float f[HEADS][8];
 #pragma unroll
     for (int j = 0; j < HEADS; ++j) {
@@ -167,7 +167,7 @@ __global__ void __launch_bounds__(kThreads, HEADS == 4 ? 8 : 10) attn_append_ker
         uint8_t* base = is_v ? p.kv.v : p.kv.k;
         if (p.kv.e4m3) {
             const float* sc = is_v ? p.kv.v_scale : p.kv.k_scale;
-            const float scale = sc ? __ldg(sc + kh) : 1.f;
+            const float scale = sc ? ld_now(sc + kh) : 1.f;
             *reinterpret_cast<uint32_t*>(base + at + e0) = pack_e4m3x4(y, scale);
             *reinterpret_cast<uint32_t*>(base + at + e1) = pack_e4m3x4(y + 4, scale);
         } else {

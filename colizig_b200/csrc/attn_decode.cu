@@ -132,7 +132,7 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
 
 // The length of sequence b, bounded by its page table.
 __device__ __forceinline__ int seq_len(const AttnDecodeParams& p, int b) {
-    const int n = __ldg(p.lens + b);
+    const int n = ld_now(p.lens + b);
     const int most = (int)(p.table_width * p.kv.page_size);
     return n < 0 ? 0 : n > most ? most : n;
 }
@@ -265,7 +265,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) attn_decode_kernel(const __gri
     uint32_t sum[6] = {0, 0, 0, 0, 0, 0};
     auto count = [&](int b) {
         const int l = seq_len(p, b);
-        if (blockIdx.x == 0 && (warp == 0 || p.B > 32) && __ldg(p.lens + b) != l) atomicOr(p.err, kAttnErrIndex);
+        if (blockIdx.x == 0 && (warp == 0 || p.B > 32) && ld_now(p.lens + b) != l) atomicOr(p.err, kAttnErrIndex);
         const uint32_t n = (uint32_t)(l + C::TS - 1) / C::TS;
         sum[0] += n ? n + kItemSteps : 0;
         sum[1] += (n + kWarps - 1) / kWarps;
@@ -434,7 +434,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) attn_decode_kernel(const __gri
                 const uint32_t tk = pt0 + lane * 16;
                 const uint32_t idx = tk / p.kv.page_size;
                 nxt.row = (int)(tk - idx * p.kv.page_size);
-                nxt.page = (int)tk < pt1 ? __ldg(p.table + (uint64_t)pb * p.table_stride + idx) : 0;
+                nxt.page = (int)tk < pt1 ? ld_now(p.table + (uint64_t)pb * p.table_stride + idx) : 0;
                 pt0 += SPB * C::TS;
             }
         }
@@ -474,7 +474,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) attn_decode_kernel(const __gri
         const int kh = item / (int)A.tiles, head0 = (item % (int)A.tiles) * NT * 8;
         const int heads = min(NT * 8, (int)A.group - head0);  // of this pass
         const uint64_t hbase = (uint64_t)kh * A.group + head0;
-        const float ks = p.kv.k_scale ? __ldg(p.kv.k_scale + kh) : 1.f;
+        const float ks = p.kv.k_scale ? ld_now(p.kv.k_scale + kh) : 1.f;
 
         // q as the B operand.  E4M3 caches multiply in f16, which holds every E4M3 value; q (bf16)
         // goes there as q 2^-e, e the exponent of the head's largest element: exact but for elements
@@ -491,7 +491,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) attn_decode_kernel(const __gri
 #pragma unroll
                     for (int j = 0; j < 2; ++j)
                         qf[n][k][j] =
-                            used ? __ldg(reinterpret_cast<const uint32_t*>(qr + k * 16 + j * 8 + t4 * 2)) : 0u;
+                            used ? ld_now(reinterpret_cast<const uint32_t*>(qr + k * 16 + j * 8 + t4 * 2)) : 0u;
                 ct[n][0] = ct[n][1] = p.scale * 1.4426950408889634f;
             } else {
                 // the four bytes a lane gets of a key chunk are dims 4 t4 .. 4 t4 + 3: so here too
@@ -499,7 +499,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) attn_decode_kernel(const __gri
                 uint32_t big = 0;
 #pragma unroll
                 for (int k = 0; k < KS; ++k) {
-                    rq[k] = used ? __ldg(reinterpret_cast<const uint2*>(qr + k * 16 + t4 * 4)) : make_uint2(0u, 0u);
+                    rq[k] = used ? ld_now(reinterpret_cast<const uint2*>(qr + k * 16 + t4 * 4)) : make_uint2(0u, 0u);
                     big = max(max(big, rq[k].x & 0x7fffu), (rq[k].x >> 16) & 0x7fffu);
                     big = max(max(big, rq[k].y & 0x7fffu), (rq[k].y >> 16) & 0x7fffu);
                 }
@@ -694,7 +694,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) attn_decode_kernel(const __gri
                 l[n][1] += __shfl_xor_sync(0xffffffffu, l[n][1], d);
             }
         if (t0 == 0 && t1 == len) {  // the whole item: out
-            const float vscale = p.kv.v_scale ? __ldg(p.kv.v_scale + kh) : 1.f;
+            const float vscale = p.kv.v_scale ? ld_now(p.kv.v_scale + kh) : 1.f;
             uint16_t* out = p.out + ((uint64_t)b * p.q_heads + hbase) * D;
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
@@ -750,7 +750,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) attn_decode_kernel(const __gri
     auto finish = [&](const Rec& r, int n, float* acc, float ll) {
         const int kh = r.item / (int)A.tiles, h = (r.item % (int)A.tiles) * NT * 8 + n * 8 + jh;
         if (h >= (int)A.group || !on) return;
-        const float vscale = p.kv.v_scale ? __ldg(p.kv.v_scale + kh) : 1.f;
+        const float vscale = p.kv.v_scale ? ld_now(p.kv.v_scale + kh) : 1.f;
         const float f = ll > 0.f || ll != ll ? vscale / ll : 0.f;
         uint32_t* dst = reinterpret_cast<uint32_t*>(
             p.out + ((uint64_t)r.b * p.q_heads + (uint64_t)kh * A.group + h) * D + jd);

@@ -205,9 +205,9 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
 
 // A sequence's bounds; false (and reported) when they leave the buffers.
 __device__ __forceinline__ bool bounds(const AttnPrefillParams& p, int b, int& q0, int& nq, int& k0, int& nk) {
-    q0 = __ldg(p.cu_q + b);
-    k0 = __ldg(p.cu_k + b);
-    const int q1 = __ldg(p.cu_q + b + 1), k1 = __ldg(p.cu_k + b + 1);
+    q0 = ld_now(p.cu_q + b);
+    k0 = ld_now(p.cu_k + b);
+    const int q1 = ld_now(p.cu_q + b + 1), k1 = ld_now(p.cu_k + b + 1);
     nq = q1 - q0;
     nk = k1 - k0;
     if (q0 < 0 || q1 < q0 || q1 > p.Tq || k0 < 0 || k1 < k0 || k1 > p.Tk) {

@@ -271,6 +271,40 @@ static __device__ __noinline__ bool wait_geq_bounded(const uint32_t* p, uint32_t
 // against 29.7, eleven packed prompts 57.5 against 52.5.)
 CZ_DEV void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
+// Loads for such kernels: whatever a kernel before them may have written is read by these, not by __ldg, whose
+// non-coherent path is for data that nobody writes while the kernel is resident, and which the compiler may move
+// over the wait.
+CZ_DEV int32_t ld_now(const int32_t* p) {
+    int32_t v;
+    asm volatile("ld.global.s32 %0, [%1];" : "=r"(v) : "l"(p));
+    return v;
+}
+CZ_DEV uint32_t ld_now(const uint32_t* p) {
+    uint32_t v;
+    asm volatile("ld.global.u32 %0, [%1];" : "=r"(v) : "l"(p));
+    return v;
+}
+CZ_DEV int64_t ld_now(const int64_t* p) {
+    long long v;
+    asm volatile("ld.global.s64 %0, [%1];" : "=l"(v) : "l"(p));
+    return v;
+}
+CZ_DEV float ld_now(const float* p) {
+    float v;
+    asm volatile("ld.global.f32 %0, [%1];" : "=f"(v) : "l"(p));
+    return v;
+}
+CZ_DEV uint2 ld_now(const uint2* p) {
+    uint2 v;
+    asm volatile("ld.global.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
+    return v;
+}
+CZ_DEV float4 ld_now(const float4* p) {
+    float4 v;
+    asm volatile("ld.global.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "l"(p));
+    return v;
+}
+
 // ---- warp reductions ------------------------------------------------------
 CZ_DEV float warp_sum(float v) {
 #pragma unroll

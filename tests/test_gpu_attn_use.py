@@ -8,7 +8,7 @@ import pytest
 
 torch = pytest.importorskip("torch")
 
-from colizig_b200 import ColizigError, attn, gpu  # noqa: E402
+from colizig_b200 import ColizigError, attn, gpu, moe, synth  # noqa: E402
 from tests.test_gpu_attn import Paged, close, gen, prefill_want, prompts, randn  # noqa: E402,F401
 
 pytestmark = pytest.mark.gpu
@@ -166,3 +166,61 @@ def test_decode_after_kernels_that_fill_shared_memory():
         attn.prefill(x, k, v, cu[0])
         assert torch.equal(plan.run(q, pg.table, pg.len_t), want)
     assert reported() == 0
+
+
+def test_calls_read_what_the_kernel_just_before_them_wrote():
+    """The MoE decode kernel lets the kernel after it come before it has written anything. Its experts' numbers serve as
+    decode's lengths and its output as the cache write's projections, both right behind it in a replayed graph."""
+    gpu.init()
+    g = gen(76)
+    d = synth.CONFIGS["c1"]
+    layer = moe.Layer.from_weights(830, d, synth.make_layer(d, seed=9, device="cuda"))
+    try:
+        x = synth.make_tokens(3, d.hidden, 1, device="cuda")
+        out, idx = torch.empty((3, d.hidden), device="cuda"), torch.zeros((3, d.topk), dtype=torch.int32, device="cuda")
+        gates = torch.empty((3, d.topk), device="cuda")
+        lens = idx.view(-1)
+        pg = Paged(g, [15] * lens.numel(), 2, 64, 16)
+        q = randn(g, lens.numel(), 6, 64, dtype=torch.bfloat16)
+        plan = attn.DecodePlan(pg.cache, 6, lens.numel())
+        o = plan.run(q, pg.table, lens)
+        cache = attn.KvCache.empty(1, 1, 16, 64)
+        heads = out.view(3, 4, 64)
+        slots = torch.arange(3, device="cuda")
+        qo = attn.append(cache, heads[:, :2], heads[:, 2:3], heads[:, 3:], None, slots)[0]
+
+        def both(first):
+            moe.forward(layer, x, out, idx, gates)
+            if first:
+                plan.run(q, pg.table, lens, out=o)
+            else:
+                attn.append(cache, heads[:, :2], heads[:, 2:3], heads[:, 3:], None, slots, q_out=qo)
+
+        graphs = []
+        for first in (True, False):
+            both(first)
+            torch.cuda.synchronize()
+            graphs.append(torch.cuda.CUDAGraph())
+            with torch.cuda.graph(graphs[-1]):
+                both(first)
+        seen = set()
+        for i in range(20):
+            x.copy_(synth.make_tokens(3, d.hidden, 100 + i, device="cuda"))
+            graphs[0].replay()
+            torch.cuda.synchronize()
+            n = lens.tolist()
+            seen.update(n)
+            cut = Paged.__new__(Paged)
+            cut.lens, cut.hk, cut.rows = n, pg.hk, [r[:, :k] for r, k in zip(pg.rows, n)]
+            close(o, *cut.want(q, 64 ** -0.5))
+            graphs[1].replay()
+            torch.cuda.synchronize()
+            assert torch.equal(qo, heads[:, :2].bfloat16())
+            assert torch.equal(cache.k[0, 0, :3], heads[:, 2].bfloat16())
+            assert torch.equal(cache.v[0, 0, :3], heads[:, 3].bfloat16())
+        assert len(seen) > 8
+        moe.check()
+        assert reported() == 0
+        del graphs
+    finally:
+        layer.unregister()
