@@ -44,6 +44,12 @@ constexpr uint32_t kTmemCols = 512;
 // above it: P and l then grow to at most 2^8, far inside f32 and bf16, and most tiles
 // rescale nothing.  The result does not depend on it (o and l share the factor).
 constexpr float kSlack = 8.f;
+// P = 2^(c S - c m) is one FMA with c m rounded, which moves a tile's weights by up to 2^-13 of themselves where c m is
+// this large (and past 2^31 the rounding alone overflows the exponential).  Beyond it, which trained weights do not
+// reach, m is taken off the scores in TMEM first and they are loaded again.  The code for it costs the others 0.2 of
+// 6.0 us on a prompt of 77 tokens, 1-2 % on eleven packed ones, nothing on 8,192 tokens (subtracted in registers, or as a
+// second form of the loop behind a branch: 0.2 us, 2-4 % and 2 %).
+constexpr float kPlain = 4096.f;
 
 struct PrefillArgs {
     CUtensorMap qmap, kmap, vmap;  // [rows][heads][D] in boxes of 64 columns
@@ -620,6 +626,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefill_kernel(const __grid_
             const int lim0 = tok + w.nk - w.nq;  // the tile's first token's limit
             const int lim = live ? t + w.nk - w.nq : 0x7fffffff;
             float m = -INFINITY, l = 0.f;
+            bool big = false;  // some row's maximum is past kPlain
 #pragma unroll 1
             for (int j = 0; j < tiles; ++j) {
                 ok = __all_sync(0xffffffffu, wait_bar(&B.sfull[i], sphase, abort));
@@ -630,40 +637,60 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefill_kernel(const __grid_
                 sphase ^= 1;
                 fence_after();
                 uint32_t sv[kKeys];
-#pragma unroll
-                for (int x = 0; x < 4; ++x) ld32(sv + x * 32, sa + x * 32);
-                wait_ld();
-                if (j * kKeys + kKeys - 1 > lim0) {
-                    const int cut = lim - j * kKeys;  // columns past it are not seen
-#pragma unroll
-                    for (int x = 0; x < kKeys; ++x)
-                        if (x > cut) sv[x] = 0xff800000u;
-                }
-                float mx[4] = {m, m, m, m};
-#pragma unroll
-                for (int x = 0; x < kKeys; x += 8)
-#pragma unroll
-                    for (int y = 0; y < 4; ++y)
-                        mx[y] = max3(mx[y], __uint_as_float(sv[x + 2 * y]), __uint_as_float(sv[x + 2 * y + 1]));
-                const float top = max3(mx[0], mx[1], max3(mx[2], mx[2], mx[3]));
-                if (j == 0) {
-                    m = top;
-                } else if (__any_sync(0xffffffffu, live && !((top - m) * c <= kSlack))) {
-                    // the products into O behind this tile's S have finished: S's completion covers them
-                    const float a = top == m ? 1.f : ex2((m - top) * c);
-                    m = top;
-                    l *= a;
+                float mc = 0.f;
 #pragma unroll 1
-                    for (int x = 0; x < D / 16; ++x) {
-                        uint32_t o[16];
-                        ld16(o, oa + x * 16);
+                for (bool again = false;; again = true) {
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) ld32(sv + x * 32, sa + x * 32);
+                    wait_ld();
+                    if (j * kKeys + kKeys - 1 > lim0) {
+                        const int cut = lim - j * kKeys;  // columns past it are not seen
+#pragma unroll
+                        for (int x = 0; x < kKeys; ++x)
+                            if (x > cut) sv[x] = 0xff800000u;
+                    }
+                    if (again) break;
+                    float mx[4] = {m, m, m, m};
+#pragma unroll
+                    for (int x = 0; x < kKeys; x += 8)
+#pragma unroll
+                        for (int y = 0; y < 4; ++y)
+                            mx[y] = max3(mx[y], __uint_as_float(sv[x + 2 * y]), __uint_as_float(sv[x + 2 * y + 1]));
+                    const float top = max3(mx[0], mx[1], max3(mx[2], mx[2], mx[3]));
+                    if (j == 0) {
+                        m = top;
+                        big = __any_sync(0xffffffffu, live && fabsf(m * c) > kPlain);
+                    } else if (__any_sync(0xffffffffu, live && !((top - m) * c <= kSlack))) {
+                        // the products into O behind this tile's S have finished: S's completion covers them
+                        const float a = top == m ? 1.f : ex2((m - top) * c);
+                        m = top;
+                        big = __any_sync(0xffffffffu, live && fabsf(m * c) > kPlain);
+                        l *= a;
+#pragma unroll 1
+                        for (int x = 0; x < D / 16; ++x) {
+                            uint32_t o[16];
+                            ld16(o, oa + x * 16);
+                            wait_ld();
+#pragma unroll
+                            for (int y = 0; y < 16; ++y) o[y] = __float_as_uint(__uint_as_float(o[y]) * a);
+                            st16(oa + x * 16, o);
+                        }
+                    }
+                    mc = m == -INFINITY ? 0.f : m * c;
+                    if (!big) break;
+                    const float less = fabsf(mc) > kPlain ? m : 0.f;
+#pragma unroll 1
+                    for (int x = 0; x < kKeys / 16; ++x) {
+                        uint32_t t[16];
+                        ld16(t, sa + x * 16);
                         wait_ld();
 #pragma unroll
-                        for (int y = 0; y < 16; ++y) o[y] = __float_as_uint(__uint_as_float(o[y]) * a);
-                        st16(oa + x * 16, o);
+                        for (int y = 0; y < 16; ++y) t[y] = __float_as_uint(__uint_as_float(t[y]) - less);
+                        st16(sa + x * 16, t);
                     }
+                    wait_st();
+                    if (less != 0.f) mc = 0.f;
                 }
-                const float mc = m == -INFINITY ? 0.f : m * c;
                 const f2 cc = pair(c, c), mm = pair(-mc, -mc);
                 f2 sum0 = 0, sum1 = 0;
 #pragma unroll

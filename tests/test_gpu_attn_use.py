@@ -224,3 +224,43 @@ def test_calls_read_what_the_kernel_just_before_them_wrote():
         del graphs
     finally:
         layer.unregister()
+
+
+def one_key_each(g, n, d):
+    """n keys of random signs: a key as a query has d as its product with itself and at most d - 2 with the others."""
+    signs = torch.randint(0, 2, (n, d), generator=g, device="cuda") * 2 - 1
+    return signs.to(torch.bfloat16)
+
+
+@pytest.mark.parametrize("big", [2.0 ** 8, 2.0 ** 15, 2.0 ** 30, 2.0 ** 55])
+@pytest.mark.parametrize("d", [64, 128])
+def test_prefill_scores_of_any_size(big, d):
+    """Scores far beyond those of trained weights, over several key tiles and rescalings: softmax leaves each query its
+    one best key. (Signs times powers of two: the products are exact, two scores differ by 2 big^2 scale or not at
+    all.)"""
+    g = gen(77)
+    n, hk, group = 700, 2, 4
+    k = one_key_each(g, n * hk, d).view(n, hk, d)
+    pick = (torch.rand((n, hk, group), generator=g, device="cuda") * (torch.arange(n, device="cuda")[:, None, None] + 1)).long()
+    q = torch.stack([k[pick[:, h], h] for h in range(hk)], 1).reshape(n, hk * group, d)
+    v = randn(g, n, hk, d, dtype=torch.bfloat16)
+    cu = torch.tensor([0, n], dtype=torch.int32, device="cuda")
+    q, k = q * big, k * big
+    got = attn.prefill(q, k, v, cu)
+    close(got, *prefill_want(q, k, v, [n], [n], d ** -0.5))
+
+
+@pytest.mark.parametrize("big", [2.0 ** 8, 2.0 ** 30, 2.0 ** 55])
+def test_decode_scores_of_any_size(big):
+    g = gen(78)
+    pg = Paged(g, [900, 33], 2, 128, 64)
+    for b, rows in enumerate(pg.rows):
+        n = rows.shape[1]
+        k = one_key_each(g, n * 2, 128).view(n, 2, 128) * big
+        rows[0] = k.double()
+        for i in range(-(-n // 64)):
+            m = min(64, n - 64 * i)
+            pg.cache.k[int(pg.table[b, i]), :, :m] = k[64 * i: 64 * i + m].transpose(0, 1)
+    q = torch.stack([pg.rows[b][0][at].repeat_interleave(4, 0) for b, at in enumerate((611, 32))]).to(torch.bfloat16)
+    got = attn.DecodePlan(pg.cache, 8, 2).run(q, pg.table, pg.len_t)
+    close(got, *pg.want(q, 128 ** -0.5))
