@@ -76,12 +76,12 @@ def _mark(s, *tensors) -> None:
             t.record_stream(s)
 
 
-def _room(s, t: Optional[torch.Tensor], shape, device):
-    """An output for work on stream s: given, or allocated there."""
-    if t is not None:
+def _room(s, t: Optional[torch.Tensor], like, device):
+    """An output for work on stream s: given, or allocated there in `like`'s shape."""
+    if t is not None or not isinstance(like, torch.Tensor):  # (what is no tensor is refused by the call itself)
         return t
     with torch.cuda.stream(s):
-        return torch.empty(shape, dtype=torch.bfloat16, device=device)
+        return torch.empty(like.shape, dtype=torch.bfloat16, device=device)
 
 
 def _need(ok: bool, what: str) -> None:
@@ -161,9 +161,9 @@ def append(cache: KvCache, q, k, v, positions, slots, rope=None, q_norm=None, k_
         if s is not None:
             _mark(s, q, k, v, positions, slots, rope, q_norm, k_norm, cache.k, cache.v, cache.k_scale, cache.v_scale, q_out,
                   k_out, v_out)
-            q_out = _room(s, q_out, q.shape, cache.device)
-            k_out = _room(s, k_out, k.shape, cache.device) if packed else k_out
-            v_out = _room(s, v_out, v.shape, cache.device) if packed else v_out
+            q_out = _room(s, q_out, q, cache.device)
+            k_out = _room(s, k_out, k, cache.device) if packed else k_out
+            v_out = _room(s, v_out, v, cache.device) if packed else v_out
     r = cache._lib.append(cache._at, dev, q, k, v, positions, slots, rope, q_norm, k_norm, eps, packed, q_out, k_out, v_out,
                           handle)
     if r.__class__ is int:
@@ -200,7 +200,7 @@ class DecodePlan:
         handle, s = (_current(dev), None) if stream is None else _elsewhere(stream, dev)
         if s is not None:
             _mark(s, q, table, lens, out, c.k, c.v, c.k_scale, c.v_scale, self._ws)
-            out = _room(s, out, q.shape, c.device)
+            out = _room(s, out, q, c.device)
         elif handle != self._home:  # the plan may be dropped while the call runs
             self._ws.record_stream(torch.cuda.current_stream(dev))
         r = c._lib.decode(c._at, dev, self.q_heads, self.max_batch, self.scale, self._wsp, q, table, lens, out, handle)
@@ -215,19 +215,21 @@ def prefill(q, k, v, cu_q, cu_k=None, scale: Optional[float] = None, out=None, s
     strides free; cu i32 [B + 1], cu_k defaults to cu_q).  Queries are the last tokens of
     their sequence; a query that sees no key gives zeros; rows past the last sequence's are not written.  scale
     defaults to head_dim ** -0.5."""
+    if not isinstance(q, torch.Tensor):
+        raise ValueError(f"q must be a tensor, got {type(q).__name__}")
     dev = q.get_device()
     if dev < 0:
         raise ValueError(f"q must be a CUDA tensor, got one on {q.device}")
     _ready(dev)
     if scale is None:
-        scale = q.shape[-1] ** -0.5
+        scale = q.shape[2] ** -0.5 if q.dim() == 3 and q.shape[2] else 1.0  # (other shapes are refused below)
     if stream is None:
         handle = _current(dev)
     else:
         handle, s = _elsewhere(stream, dev)
         if s is not None:
             _mark(s, q, k, v, cu_q, cu_k, out)
-            out = _room(s, out, q.shape, q.device)
+            out = _room(s, out, q, q.device)
     r = _native().prefill(dev, q, k, v, cu_q, cu_k, scale, out, handle)
     if r.__class__ is int:
         _abi.check("colizig_cuda_attn_prefill", r)

@@ -137,3 +137,25 @@ def test_check_waits_for_a_stream_of_the_library_s_device(monkeypatch):
     attn.check()
     attn.check(stream=7)
     assert seen == [1003, 7]
+
+
+@pytest.mark.parametrize("elsewhere", [False, True])
+@pytest.mark.parametrize("q", [None, 3, [paper(2, 4, 128)], paper(), paper(2, 4, 0), paper(2, 4, 96)])
+def test_queries_that_are_no_rows_of_heads_are_refused(on_paper, monkeypatch, q, elsewhere):
+    """ValueError, on the current stream and on a given one."""
+    cache, plan, done = on_paper
+    kw = {}
+    if elsewhere:
+        monkeypatch.setattr(attn, "_elsewhere", lambda stream, index: (stream, contextlib.nullcontext()))
+        monkeypatch.setattr(attn, "_mark", lambda *a: None)
+        monkeypatch.setattr(torch.cuda, "stream", lambda s: s)
+        monkeypatch.setattr(torch, "empty", lambda shape, **k: paper(*shape))
+        kw = {"stream": 5}
+    kv, i32 = paper(2, 2, 128), paper(2, dtype=torch.int32)
+    with pytest.raises(ValueError, match="q must be"):
+        attn.prefill(q, kv, kv, i32, **kw)
+    with pytest.raises(ValueError, match="q must be"):
+        plan.run(q, paper(2, 3, dtype=torch.int32), i32, **kw)
+    with pytest.raises(ValueError, match="q must be"):
+        attn.append(cache, q, kv, kv, None, paper(2, dtype=torch.int64), **kw)
+    assert not done
