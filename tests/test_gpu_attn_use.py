@@ -9,7 +9,7 @@ import pytest
 torch = pytest.importorskip("torch")
 
 from colizig_b200 import ColizigError, attn, gpu, moe, synth  # noqa: E402
-from tests.test_gpu_attn import Paged, close, gen, prefill_want, prompts, randn  # noqa: E402,F401
+from tests.test_gpu_attn import Paged, close, gen, prefill_want, prompts, randn, softmax_rows  # noqa: E402,F401
 
 pytestmark = pytest.mark.gpu
 
@@ -264,3 +264,102 @@ def test_decode_scores_of_any_size(big):
     q = torch.stack([pg.rows[b][0][at].repeat_interleave(4, 0) for b, at in enumerate((611, 32))]).to(torch.bfloat16)
     got = attn.DecodePlan(pg.cache, 8, 2).run(q, pg.table, pg.len_t)
     close(got, *pg.want(q, 128 ** -0.5))
+
+
+def test_two_plans_at_once_on_two_streams():
+    a, b = long_one(gen(80)), long_one(gen(81), n=9001, hq=12, hk=4, d=64)
+    plans = [attn.DecodePlan(pg.cache, q.shape[1], 1) for pg, q, _ in (a, b)]
+    streams = [torch.cuda.Stream() for _ in plans]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(40):
+        for (pg, q, _), plan, s in zip((a, b), plans, streams):
+            got.append(plan.run(q, pg.table, pg.len_t, stream=s))
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, (a, b)[i % 2][2]) for i, o in enumerate(got))
+    assert reported() == 0
+
+
+def test_two_threads_with_a_plan_and_a_stream_each():
+    ones = [long_one(gen(82)), long_one(gen(83), n=9001, hq=12, hk=4, d=64)]
+    x, k, v, cu = prompts(gen(84), [500, 33], [500, 33], 8, 2, 64, False)
+    whole = attn.prefill(x, k, v, cu[0])
+    torch.cuda.synchronize()
+    good = [0, 0]
+
+    def work(i):
+        pg, q, want = ones[i]
+        s = torch.cuda.Stream()
+        with torch.cuda.stream(s):
+            plan = attn.DecodePlan(pg.cache, q.shape[1], 1)
+            outs = [(plan.run(q, pg.table, pg.len_t), attn.prefill(x, k, v, cu[0])) for _ in range(60)]
+            s.synchronize()
+            good[i] = sum(torch.equal(o, want) and torch.equal(p, whole) for o, p in outs)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert good == [60, 60] and reported() == 0
+
+
+@pytest.mark.parametrize("nq,nk", [([64], [8192]), ([1], [5000]), ([17, 200], [4097, 300])])
+def test_prefill_of_a_short_chunk_on_many_keys(nq, nk):
+    q, k, v, cu = prompts(gen(85), nq, nk, 32, 4, 128, False)
+    got = attn.prefill(q, k, v, *cu)
+    close(got, *prefill_want(q, k, v, nq, nk, 128 ** -0.5))
+
+
+def test_a_prompt_in_chunks_through_the_cache():
+    """Each chunk's keys are appended, all of them so far read back out of the pages and attended to."""
+    g = gen(86)
+    n, hq, hk, d, page = 333, 8, 2, 64, 16
+    q, k, v, _ = prompts(g, [n], [n], hq, hk, d, False)
+    cache = attn.KvCache.empty(-(-n // page), hk, page, d)
+    order = torch.randperm(cache.pages, generator=torch.Generator().manual_seed(1)).cuda()
+    at = 0
+    for m in (100, 1, 200, 32):
+        i = torch.arange(at, at + m, device="cuda")
+        qo = attn.append(cache, q[i], k[i], v[i], None, order[i // page] * page + i % page)[0]
+        at += m
+        rows = [t[order].transpose(1, 2).reshape(-1, hk, d)[:at] for t in (cache.k, cache.v)]
+        ends = [torch.tensor([0, e], dtype=torch.int32, device="cuda") for e in (m, at)]
+        got = attn.prefill(qo, *rows, *ends)
+        close(got, *prefill_want(q[at - m: at], k[:at], v[:at], [m], [at], d ** -0.5))
+
+
+def test_decode_of_a_full_batch_on_e4m3():
+    g = gen(87)
+    lens = [1800 + 37 * i % 251 for i in range(64)]
+    pg = Paged(g, lens, 4, 128, 64, True)
+    q = randn(g, 64, 32, 128, dtype=torch.bfloat16) * 2
+    got = attn.DecodePlan(pg.cache, 32, 64).run(q, pg.table, pg.len_t)
+    close(got, *pg.want(q, 128 ** -0.5))
+
+
+def test_scores_of_minus_infinity_leave_their_keys_out():
+    """Keys of the type's lowest value, whose products with large queries are -infinity: as if they were masked; a row
+    of nothing else gives zeros."""
+    g = gen(88)
+    n, d = 300, 128
+    low = torch.finfo(torch.bfloat16).min
+    q = torch.full((1, 8, d), 4.0, device="cuda", dtype=torch.bfloat16)
+    k = randn(g, n, 1, d, dtype=torch.bfloat16)
+    v = randn(g, n, 1, d, dtype=torch.bfloat16)
+    out = torch.rand(n, generator=g, device="cuda") < 0.5
+    k[out] = low
+    o, w = softmax_rows(q[0], k[~out, 0], v[~out, 0], d ** -0.5, torch.ones(8, int((~out).sum()), dtype=torch.bool, device="cuda"))
+    cache = attn.KvCache.empty(-(-n // 16), 1, 16, d)
+    table = torch.arange(cache.pages, dtype=torch.int32, device="cuda")[None]
+    one, all_n = (torch.tensor([0, e], dtype=torch.int32, device="cuda") for e in (1, n))
+    for alone in (False, True):
+        if alone:
+            k[:] = low
+        attn.append(cache, k.expand(n, 1, d), k, v, None, torch.arange(n, device="cuda"))
+        got = [attn.DecodePlan(cache, 8, 1).run(q, table, all_n[1:]), attn.prefill(q, k, v, one, all_n)]
+        for x in got:
+            if alone:
+                assert not x.any()
+            else:
+                close(x[0], o, w)
