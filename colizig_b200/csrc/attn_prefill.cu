@@ -785,6 +785,26 @@ bool make_map(CUtensorMap* map, const uint16_t* base, uint64_t rows, uint64_t he
               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// One prompt in turns of `step` tokens: what the busiest block's turns take, in hundredths of a pair's time on a key
+// tile.  A single query tile takes 0.94 of that (0.9 with heads of 64), a further turn 1.5 of it to begin and end.
+uint64_t busiest(const AttnPrefillParams& p, int step, bool pair, int64_t heads, int num_sms) {
+    const uint64_t tile = pair ? 100 : p.head_dim == 64 ? 90 : 94;
+    const int64_t n = ((int64_t)p.Tq + step - 1) / step, turns = n * heads;
+    uint64_t most = 0;
+    for (int64_t x = 0; x < num_sms && x < turns; ++x) {
+        uint64_t sum = 0;
+        for (int64_t t = 0;; ++t) {  // as the picking warp goes: longest first, in turn from either end
+            const int64_t item = t * num_sms + (t & 1 ? num_sms - 1 - x : x);
+            if (item >= turns) break;
+            const int64_t end = (n - item / heads) * step;  // the turn's last query's keys
+            const int64_t keys = (end < p.Tq ? end : p.Tq) + (int64_t)p.Tk - p.Tq;
+            sum += (t ? 150 : 0) + (keys > 0 ? (uint64_t)(keys + kKeys - 1) / kKeys * tile : 0);
+        }
+        if (sum > most) most = sum;
+    }
+    return most;
+}
+
 template <int D>
 int launch(const PrefillArgs& a, uint32_t grid, cudaStream_t st) {
     static uint32_t set = 0;  // the library's lock is held
@@ -806,16 +826,19 @@ int attn_prefill_launch(const AttnPrefillParams& p, int num_sms, cudaStream_t st
     a.htiles = (a.group + 127) / 128;
     a.pack = (a.group + a.htiles - 1) / a.htiles;
     a.tokens = 128 / a.pack;
-    // Turns at most. One query tile each where that still leaves SMs idle, and for one long prompt
-    // whose pairs would: the last pair, which is the longest, then bounds the call. Measured for
-    // one prompt, single tiles against pairs: 8 heads on 1, 2,400 tokens 32.1 against 35.8 us, 4,600
-    // 58.2 against 63.2; 12 on 2, 2,500 tokens 37.1 against 40.1; but 32 on 4, 1,100 tokens 23.1
-    // against 22.0, and 4 prompts of 900 tokens in all (which then need the sort) 18.1 against 12.2.
+    // Turns at most.  One query tile each where that still leaves SMs idle.  One prompt whose pairs do: by the key tiles
+    // of the block that gets most, single against pairs (`busiest`).  Measured: 8 heads on 1 of 64, 2,400 tokens 32.6
+    // against 36.1 us, 4,600 59.7 against 64.5, but 3,000 after 3,000 keys 91.0 against 83.7; 12 on 2 of 128, 2,000
+    // tokens 31.0 against 32.8, but 2,500 after 2,500 keys 96.6 against 73.5; 32 on 4 of 128, 600 tokens 13.9 against
+    // 14.7, 900 18.8 against 18.4, but 1,100 23.3 against 21.7, 700 after 4,000 keys 111.1 against 67.5.  Several prompts
+    // of more single tiles than SMs take pairs (their lengths are on the device): 2 of 350 tokens 12.1 against 15.6.
     const uint64_t heads = (uint64_t)p.kv_heads * a.htiles;
     const uint64_t single = ((uint64_t)p.Tq / a.tokens + p.B) * heads;
     const uint64_t pairs = ((uint64_t)p.Tq / (2 * a.tokens) + p.B) * heads;
-    const bool lone = p.B == 1 && p.Tk >= 2048 && pairs <= (uint64_t)num_sms;
-    a.step = single <= (uint64_t)num_sms || lone ? a.tokens : 2 * a.tokens;
+    const uint64_t sms = (uint64_t)num_sms;
+    const auto most = [&](int step, bool pair) { return busiest(p, step, pair, (int64_t)heads, num_sms); };
+    const bool one = single <= sms || (p.B == 1 && pairs <= sms && most(a.tokens, false) < most(2 * a.tokens, true));
+    a.step = one ? a.tokens : 2 * a.tokens;
     const uint64_t turns = ((uint64_t)p.Tq / a.step + p.B) * heads;
     if (turns > 0x3fffffffu) return CZ_ESHAPE;
     a.sms = (uint32_t)num_sms;

@@ -363,3 +363,36 @@ def test_scores_of_minus_infinity_leave_their_keys_out():
                 assert not x.any()
             else:
                 close(x[0], o, w)
+
+
+def microseconds(f, n=20):
+    """Device time of a call in a replayed graph."""
+    f()
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        for _ in range(n):
+            f()
+    times = []
+    for _ in range(7):
+        a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        a.record()
+        graph.replay()
+        b.record()
+        torch.cuda.synchronize()
+        times.append(a.elapsed_time(b) * 1e3 / n)
+    return sorted(times)[3]
+
+
+@pytest.mark.parametrize("nq,nk,hq,hk,d", [(700, 4700, 32, 4, 128), (1000, 4000, 32, 4, 128), (2500, 5000, 12, 2, 128)])
+def test_a_chunk_takes_no_second_round_of_long_tiles(nq, nk, hq, hk, d):
+    """Queries after many keys, whose tiles all are long: where pairs of tiles fill the SMs once, the call takes about as
+    long as a pair alone on as many keys (an eighth of the queries), not twice that."""
+    g = gen(89)
+
+    def call(n):
+        q, k, v, cu = prompts(g, [n], [nk], hq, hk, d, False)
+        out = torch.empty_like(q)
+        return lambda: attn.prefill(q, k, v, *cu, out=out)
+
+    assert microseconds(call(nq)) < 1.6 * microseconds(call(nq // 8))
