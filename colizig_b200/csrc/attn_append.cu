@@ -16,9 +16,10 @@
 // and share the cosines and sines.
 //
 // Bound by memory: 8,192 tokens of 32 + 2 x 4 heads of 128 in f32 to bf16, with packed copies, are 272 MB
-// and take 56 us, 4.86 TB/s (0.75 of a copy's rate).  Four heads against two: 56.0 and 56.1 us there,
-// 5.9 and 6.7 us for 1,531 tokens of 16 + 32 heads of 64 in bf16; for 96 tokens 4.2 and 3.5 us, for one 3.7
-// and 3.0 us.
+// and take 54.9 us, 4.96 TB/s (0.77 of a copy's rate).  Four heads against two: 54.9 and 55.8 us there,
+// 5.4 and 6.2 us for 1,531 tokens of 16 + 32 heads of 64 in bf16; for 96 tokens 3.9 and 3.1 us, for one 3.1
+// and 2.4 us.  The launch bounds make each instance spill 24 to 80 bytes a thread; two blocks fewer an SM spill
+// nothing, but take 59.4 and 6.5 us (one token 2.2, 96 tokens 2.9): more loads in flight are worth more.
 #include <cuda_bf16.h>
 #include <cuda_fp8.h>
 #include <cuda_runtime.h>

@@ -21,8 +21,8 @@
 // go in order along the line, so results do not depend on timing.  With few or short items the
 // parts are laid so that none is cut between blocks, or as few as the idle blocks are worth.
 //
-// Measured: 96 sequences of up to 8,192 tokens, 32 heads on 4 of 128, 1.51 GB: 231-236 us, 6.42-6.55
-// TB/s (a copy's rate is 6.46); one of 32,781 tokens 21.7 us (10.4 at that rate: some 5 us pass before the
+// Measured: 96 sequences of up to 8,192 tokens, 32 heads on 4 of 128, 1.51 GB: 231-237 us, 6.39-6.55
+// TB/s (a copy's rate is 6.46); one of 32,781 tokens 22.1-22.6 us (10.4 at that rate: some 5 us pass before the
 // first keys arrive, some 5 in the joins); 97 tokens 5.7 us.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>

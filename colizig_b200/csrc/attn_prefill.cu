@@ -14,8 +14,8 @@
 // tokens.  Keys and values are read once for all of them, a short prompt still fills
 // the tile (16 tokens of 8 heads), and the diagonal wastes at most 16 of 128 keys there.
 //
-// One block per SM runs through pairs of query tiles (single ones where SMs would idle: 927 tokens of 8
-// heads on one, 21.7 -> 16.2 us), the longest first and in turn from either end, so that the blocks
+// One block per SM runs through pairs of query tiles (single ones where that takes the busiest block less: 927 tokens
+// of 8 heads on one, 21.7 -> 16.2 us), the longest first and in turn from either end, so that the blocks
 // end together; the next pair's queries, keys and first products go out
 // while the last one's results are written.  Warps: 0-3 and 4-7 softmax of query tile 0 and 1 (a
 // thread a row), 8 TMA loads, 9 MMA issue, 10 picks the pairs, 11 clears what lies behind the last

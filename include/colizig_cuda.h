@@ -320,7 +320,10 @@ int colizig_cuda_debug_watch_wait(int (*query)(void*), int (*async_error)(void*)
  *
  * Indices that live in device memory (positions, slots, page tables, lengths, sequence
  * bounds) are checked by the kernels: one that points outside its buffer is never
- * followed, and the call sets a word that colizig_cuda_attn_check reports as -11. */
+ * followed (a page is read as page 0, a position as 0, a length is cut to the page table, a
+ * slot or a sequence is left out), and the call sets a word that colizig_cuda_attn_check
+ * reports as -11.  The word is one for all calls, streams and threads of the process and
+ * outlives a shutdown (a graph replayed after the next init reports there). */
 
 #define COLIZIG_KV_BF16 0u
 #define COLIZIG_KV_E4M3 1u
@@ -368,9 +371,11 @@ int colizig_cuda_attn_append(const colizig_kv_cache* cache, const void* q, const
  * head_dim] at q_stride elements a sequence, table int32 [B, table_width] at
  * table_stride, lens int32 [B]; out bf16 [B, q_heads, head_dim].  A sequence of length 0
  * gives zeros.  Rows of a page past the length may hold anything, NaN included.
- * B is at most COLIZIG_ATTN_MAX_BATCH, and B * kv_heads * table_width * page_size / 16 under 2^31 (else -8).  workspace: colizig_cuda_attn_decode_workspace
- * bytes, 256-byte aligned and zeroed once before its first use; each call leaves it
- * ready for the next.  Calls that may overlap in time need a workspace each. */
+ * B is at most COLIZIG_ATTN_MAX_BATCH, and B * kv_heads * table_width * page_size / 16
+ * under 2^31 (else -8).  workspace: colizig_cuda_attn_decode_workspace bytes, 256-byte
+ * aligned and zeroed once before its first use (in an order that the first call's stream
+ * sees); each call leaves it ready for the next.  Calls that may overlap in time need a
+ * workspace each. */
 #define COLIZIG_ATTN_MAX_BATCH 4096
 size_t colizig_cuda_attn_decode_workspace(void);
 int colizig_cuda_attn_decode(const colizig_kv_cache* cache, const void* q, uint64_t q_stride, int B,
@@ -391,9 +396,9 @@ int colizig_cuda_attn_prefill(const void* q, const void* k, const void* v, uint6
                               uint32_t head_dim, const int32_t* cu_q, const int32_t* cu_k, float scale, void* out,
                               void* stream);
 
-/* Reads and clears the attention calls' error word (synchronises `stream`): 0, -11 when a
- * call since the last read met an index outside its buffer, -7 when a bounded wait in
- * a kernel gave up. */
+/* Takes the attention calls' error word and leaves 0, in one step (synchronises `stream`;
+ * what other streams report later stays for the next read): 0, -11 when a call since the
+ * last read met an index outside its buffer, -7 when a bounded wait in a kernel gave up. */
 int colizig_cuda_attn_check(void* stream);
 
 #ifdef __cplusplus
