@@ -28,11 +28,11 @@ def test_a_small_layer_on_512_bytes_keeps_the_grouped_path():
     d = moe.Dims(hidden=256, experts=4, topk=2, inter=128)
     w = synth.make_layer(d, seed=5, device="cuda")
     x = synth.make_tokens(64, d.hidden, 2, device="cuda")
-    room = 440 * 1024  # what the layer takes, and some
+    room = 400 * 1024  # what the layer takes, and a little
     held, layers = [], []
     try:
         for _ in range(200):
-            held.append(block(256))
+            held.append(block(room + 512))  # the next block of this hole lies 512 bytes further on
             at = block(room)
             rt.cudaFree(at)
             if at % 1024:
